@@ -340,7 +340,7 @@ def _plain_plan(s):
     place = lens[seq] + t - (ends - step)[seq]
     live = (t < ends[-1]) & good
     slot = table[seq, (place // page).clamp(0, wide - 1)] * page + place % page
-    return {'lens': torch.where(good, after, lens).int(), 'cu': torch.cat([ends.new_zeros(1), ends]).int(), 'slots': torch.where(live, slot, -1).int(),
+    return {'lens': torch.where(good, after, lens).int(), 'cu': torch.where(good, torch.cat([ends.new_zeros(1), ends]), 0).int(), 'slots': torch.where(live, slot, -1).int(),
             'places': torch.where(live, place, -1).int(),
             'ring_state': torch.where(good, torch.stack([(state[0] + took[-1]) % blocks, state[1] - took[-1] + gave[-1]]), state).int(),
             'status': status.int().reshape(1), 'table': table, 'ring': ring}
