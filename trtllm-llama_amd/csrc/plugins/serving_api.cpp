@@ -1,0 +1,195 @@
+// extern "C" surface of include/tllm_serving_api.h: every size, type, stride and alignment that a kernel relies on is checked here, on the host,
+// before anything is launched.  What only the device knows (lengths, table entries, slots) the kernels check themselves.
+#include "../kernels/serving_kernels.h"
+#include <exception>
+#include <initializer_list>
+
+using namespace tllm;
+using namespace tllm::kernels;
+
+namespace
+{
+bool is_page(int32_t v)
+{
+    return v == 16 || v == 32 || v == 64 || v == 128;
+}
+
+bool is_head(int32_t v)
+{
+    return v == 64 || v == 128 || v == 256;
+}
+
+bool aligned(const void* p, size_t to)
+{
+    return reinterpret_cast<uintptr_t>(p) % to == 0;
+}
+
+constexpr int32_t kMaxRows = 1 << 19, kMaxHeads = 1024;
+
+#define TLLM_REFUSE(cond, ...)                                                                                         \
+    do                                                                                                                 \
+    {                                                                                                                  \
+        if (cond)                                                                                                      \
+        {                                                                                                              \
+            set_error(__VA_ARGS__);                                                                                    \
+            return false;                                                                                              \
+        }                                                                                                              \
+    } while (0)
+
+bool plan_fits(const tllm_paged_plan_params_t* p)
+{
+    const char* const me = "tllm_paged_plan";
+    TLLM_REFUSE(!p, "%s: null parameters", me);
+    TLLM_REFUSE(p->n_seqs < 1 || p->n_seqs > kPlanMaxSeqs, "%s: n_seqs %d outside [1, %d]", me, p->n_seqs, kPlanMaxSeqs);
+    TLLM_REFUSE(p->n_rows < 0 || p->n_rows > kMaxRows, "%s: n_rows %d outside [0, %d]", me, p->n_rows, kMaxRows);
+    TLLM_REFUSE(!is_page(p->page_size), "%s: page_size %d is none of 16, 32, 64, 128", me, p->page_size);
+    TLLM_REFUSE(p->num_blocks < 1 || (int64_t) p->num_blocks * p->page_size > INT32_MAX, "%s: num_blocks %d: 1 or more, times page_size below 2^31", me, p->num_blocks);
+    TLLM_REFUSE(p->max_blocks < 1 || p->max_blocks > kMaxRows, "%s: max_blocks %d outside [1, %d]", me, p->max_blocks, kMaxRows);
+    TLLM_REFUSE(p->table_stride < p->max_blocks, "%s: table_stride %lld is less than max_blocks %d", me, (long long) p->table_stride, p->max_blocks);
+    TLLM_REFUSE(!p->lens || !p->new_lens || !p->ring || !p->ring_state || !p->block_table || !p->cu_tokens || !p->lens_out || !p->ring_state_out || !p->status
+            || (p->n_rows && (!p->slot_map || !p->positions)),
+        "%s: null tensor", me);
+    for (const void* t : std::initializer_list<const void*>{p->lens, p->new_lens, p->ring, p->ring_state, p->block_table, p->cu_tokens, p->slot_map, p->positions, p->lens_out,
+             p->ring_state_out, p->status})
+        TLLM_REFUSE(!aligned(t, 4), "%s: a tensor is not 4-byte aligned", me);
+    return true;
+}
+
+bool rows_fit(const char* me, const char* what, const void* t, int64_t row, int64_t head)
+{
+    TLLM_REFUSE(!t, "%s: null %s", me, what);
+    TLLM_REFUSE(!aligned(t, 16) || row % 8 || head % 8, "%s: %s has to be 16-byte aligned, with strides that are multiples of 8 elements", me, what);
+    return true;
+}
+
+bool cache_fits(const char* me, int32_t dtype, int32_t cache_type, int32_t head_size, int32_t page_size, int32_t num_blocks, int32_t kv_heads, const void* pool, const float* scales)
+{
+    TLLM_REFUSE(dtype != TLLM_HALF && dtype != TLLM_BF16, "%s: dtype %d is neither float16 nor bfloat16", me, dtype);
+    TLLM_REFUSE(cache_type != TLLM_INT8 && cache_type != TLLM_FP8, "%s: cache_type %d is neither int8 nor fp8", me, cache_type);
+    TLLM_REFUSE(!is_head(head_size), "%s: head_size %d is none of 64, 128, 256", me, head_size);
+    TLLM_REFUSE(!is_page(page_size), "%s: page_size %d is none of 16, 32, 64, 128", me, page_size);
+    TLLM_REFUSE(num_blocks < 1 || (int64_t) num_blocks * page_size > INT32_MAX, "%s: num_blocks %d: 1 or more, times page_size below 2^31", me, num_blocks);
+    TLLM_REFUSE(kv_heads < 1 || kv_heads > kMaxHeads, "%s: kv_heads %d outside [1, %d]", me, kv_heads, kMaxHeads);
+    TLLM_REFUSE(!pool || !aligned(pool, 16), "%s: the pool is null or not 16-byte aligned", me);
+    TLLM_REFUSE(!scales || !aligned(scales, 4), "%s: the scales are null or not 4-byte aligned", me);
+    return true;
+}
+
+bool append_fits(const tllm_paged_append_params_t* p)
+{
+    const char* const me = "tllm_paged_append";
+    TLLM_REFUSE(!p, "%s: null parameters", me);
+    TLLM_REFUSE(p->n_rows < 0 || p->n_rows > kMaxRows, "%s: n_rows %d outside [0, %d]", me, p->n_rows, kMaxRows);
+    if (!cache_fits(me, p->dtype, p->cache_type, p->head_size, p->page_size, p->num_blocks, p->kv_heads, p->pool, p->scales))
+        return false;
+    TLLM_REFUSE(p->q_heads < 0 || p->q_heads > kMaxHeads, "%s: q_heads %d outside [0, %d]", me, p->q_heads, kMaxHeads);
+    TLLM_REFUSE(p->rot_dim < 0 || p->rot_dim > p->head_size || p->rot_dim % 16, "%s: rot_dim %d is no multiple of 16 up to head_size %d", me, p->rot_dim, p->head_size);
+    TLLM_REFUSE(p->rope_pairs != 0 && p->rope_pairs != 1, "%s: rope_pairs %d is neither 0 nor 1", me, p->rope_pairs);
+    TLLM_REFUSE(p->rot_dim && (p->rope_len < 1 || !p->rope || !aligned(p->rope, 16)), "%s: rotation needs a 16-byte aligned rope table", me);
+    TLLM_REFUSE(p->q_heads && !p->rot_dim, "%s: queries are only rotated here, and rot_dim is 0", me);
+    if (p->n_rows == 0)
+        return true;
+    TLLM_REFUSE(!p->slot_map || !aligned(p->slot_map, 4), "%s: the slot map is null or not 4-byte aligned", me);
+    TLLM_REFUSE(p->rot_dim && (!p->positions || !aligned(p->positions, 4)), "%s: the positions are null or not 4-byte aligned", me);
+    return rows_fit(me, "k", p->k, p->k_row, p->k_head) && rows_fit(me, "v", p->v, p->v_row, p->v_head)
+        && (!p->q_heads || (rows_fit(me, "q", p->q, p->q_row, p->q_head) && rows_fit(me, "q_out", p->q_out, p->q_out_row, p->q_out_head)));
+}
+
+bool attention_fits(const tllm_paged_attention_params_t* p)
+{
+    const char* const me = "tllm_paged_attention";
+    TLLM_REFUSE(!p, "%s: null parameters", me);
+    TLLM_REFUSE(p->n_seqs < 1 || p->n_seqs > kPlanMaxSeqs, "%s: n_seqs %d outside [1, %d]", me, p->n_seqs, kPlanMaxSeqs);
+    TLLM_REFUSE(p->n_rows < 0 || p->n_rows > kMaxRows, "%s: n_rows %d outside [0, %d]", me, p->n_rows, kMaxRows);
+    if (!cache_fits(me, p->dtype, p->cache_type, p->head_size, p->page_size, p->num_blocks, p->kv_heads, p->pool, p->scales))
+        return false;
+    TLLM_REFUSE(p->q_heads < 1 || p->q_heads > kMaxHeads || p->q_heads % p->kv_heads, "%s: q_heads %d is no multiple of kv_heads %d up to %d", me, p->q_heads, p->kv_heads, kMaxHeads);
+    TLLM_REFUSE(p->max_blocks < 1 || p->max_blocks > kMaxRows, "%s: max_blocks %d outside [1, %d]", me, p->max_blocks, kMaxRows);
+    TLLM_REFUSE(p->table_stride < p->max_blocks, "%s: table_stride %lld is less than max_blocks %d", me, (long long) p->table_stride, p->max_blocks);
+    TLLM_REFUSE(p->max_new < 1 || p->max_new > kMaxRows, "%s: max_new %d outside [1, %d]", me, p->max_new, kMaxRows);
+    TLLM_REFUSE(p->max_kv < 0 || p->window < 0, "%s: a negative max_kv or window", me);
+    TLLM_REFUSE(!(p->scale > -1e30f && p->scale < 1e30f), "%s: the scale is not finite", me);
+    TLLM_REFUSE(!p->block_table || !p->cu_tokens || !p->kv_lens || !aligned(p->block_table, 4) || !aligned(p->cu_tokens, 4) || !aligned(p->kv_lens, 4),
+        "%s: tables and lengths are null or not 4-byte aligned", me);
+    TLLM_REFUSE((int64_t) p->n_seqs * p->kv_heads * (((int64_t) p->max_new * (p->q_heads / p->kv_heads) + 15) / 16) > INT32_MAX / 64
+            || (int64_t) p->n_seqs * p->max_new * p->q_heads > INT32_MAX,
+        "%s: %d requests of up to %d rows are more than one launch takes", me, p->n_seqs, p->max_new);
+    return p->n_rows == 0 || (rows_fit(me, "q", p->q, p->q_row, p->q_head) && rows_fit(me, "out", p->out, p->out_row, p->out_head));
+}
+
+bool matmul_fits(const tllm_group_matmul_params_t* p)
+{
+    const char* const me = "tllm_group_matmul";
+    TLLM_REFUSE(!p, "%s: null parameters", me);
+    TLLM_REFUSE(p->dtype != TLLM_HALF && p->dtype != TLLM_BF16, "%s: dtype %d is neither float16 nor bfloat16", me, p->dtype);
+    TLLM_REFUSE(p->group != 32 && p->group != 64 && p->group != 128, "%s: group %d is none of 32, 64, 128", me, p->group);
+    TLLM_REFUSE(p->rows < 0 || p->rows > kMaxRows, "%s: rows %d outside [0, %d]", me, p->rows, kMaxRows);
+    TLLM_REFUSE(p->n < 1 || p->n > (1 << 24) || p->k < 32 || p->k > (1 << 24) || p->k % 32, "%s: n %d, k %d: n in [1, 2^24], k a multiple of 32 up to 2^24", me, p->n, p->k);
+    TLLM_REFUSE(!p->packed || !aligned(p->packed, 16) || !p->scales || !aligned(p->scales, 16), "%s: weights or scales are null or not 16-byte aligned", me);
+    TLLM_REFUSE(p->rows && (!p->x || !aligned(p->x, 16) || p->ldx % 8 || (p->rows > 1 && p->ldx < p->k)), "%s: x has to be 16-byte aligned with a row stride that is a multiple of 8, at least k", me);
+    TLLM_REFUSE(p->rows && (!p->y || !aligned(p->y, 2) || (p->rows > 1 && p->ldy < p->n)), "%s: y is null, not 2-byte aligned or its row stride is less than n", me);
+    return true;
+}
+
+template <typename F>
+int32_t guarded(F f)
+{
+    try
+    {
+        return f() ? 1 : 0;
+    }
+    catch (const std::exception& e)
+    {
+        set_error("%s", e.what());
+        return 1;
+    }
+}
+} // namespace
+
+extern "C" {
+
+int32_t tllm_paged_plan(const tllm_paged_plan_params_t* p, tllm_stream_t stream)
+{
+    return guarded([&] { return !plan_fits(p) || launch_paged_plan(*p, reinterpret_cast<hipStream_t>(stream)); });
+}
+
+int32_t tllm_paged_append(const tllm_paged_append_params_t* p, tllm_stream_t stream)
+{
+    return guarded([&] { return !append_fits(p) || (p->n_rows && launch_paged_append(*p, reinterpret_cast<hipStream_t>(stream))); });
+}
+
+int64_t tllm_paged_attention_workspace(const tllm_paged_attention_params_t* p)
+{
+    int64_t bytes = -1;
+    if (guarded([&] {
+            if (!attention_fits(p))
+                return true;
+            bytes = p->n_rows ? (int64_t) paged_attention_workspace(*p) : 0;
+            return false;
+        }))
+        return -1;
+    return bytes;
+}
+
+int32_t tllm_paged_attention(const tllm_paged_attention_params_t* p, void* workspace, tllm_stream_t stream)
+{
+    return guarded([&] {
+        if (!attention_fits(p))
+            return true;
+        if (p->n_rows == 0)
+            return false;
+        if (paged_attention_workspace(*p) && (!workspace || !aligned(workspace, 16)))
+        {
+            set_error("tllm_paged_attention: the workspace is null or not 16-byte aligned");
+            return true;
+        }
+        return launch_paged_attention(*p, workspace, reinterpret_cast<hipStream_t>(stream)) != 0;
+    });
+}
+
+int32_t tllm_group_matmul(const tllm_group_matmul_params_t* p, tllm_stream_t stream)
+{
+    return guarded([&] { return !matmul_fits(p) || (p->rows && launch_group_matmul(*p, reinterpret_cast<hipStream_t>(stream))); });
+}
+
+} // extern "C"

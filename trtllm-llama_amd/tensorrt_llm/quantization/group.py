@@ -1,0 +1,109 @@
+"""Linear layers with 4-bit weights and a scale for each group of a row (ctypes binding of tllm_group_matmul, include/tllm_serving_api.h).
+
+Next to WeightOnlyQuantMatmul, whose 4-bit weights have one scale for a whole output channel.  y = x W^T, W[n, k] = q[n, k] s[n, k / group]."""
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from ..plugin import capi
+
+GROUPS = (32, 64, 128)
+_ACT = {torch.float16: capi.HALF, torch.bfloat16: 7}
+_ORDER = (0, 2, 4, 6, 1, 3, 5, 7)  # element of a word's eight that nibble i holds
+
+_i32, _i64, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+
+
+class _Params(ctypes.Structure):
+    _fields_ = [(n, _i32) for n in ('rows', 'n', 'k', 'group', 'dtype')] + [('ldx', _i64), ('ldy', _i64)] + [(n, _ptr) for n in ('x', 'packed', 'scales', 'y')]
+
+
+_matmul = None
+
+
+def _entry():
+    global _matmul
+    if _matmul is None:
+        f = capi.load_library().tllm_group_matmul
+        f.argtypes, f.restype = [_ptr, _ptr], _i32
+        _matmul = f
+    return _matmul
+
+
+def _checked(n: int, k: int, group: int):
+    if group not in GROUPS:
+        raise ValueError(f'group is one of {GROUPS}: got {group}')
+    if n < 1 or k < 32 or k % 32:
+        raise ValueError(f'weights are [n, k] with k a multiple of 32: got [{n}, {k}]')
+
+
+def quantize(weight: torch.Tensor, group: int, dtype=torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """weight [n, k] -> (q int8 [n, k] in -7 .. 7, scales `dtype` [n, ceil(k / group)]): the scale is the group's largest magnitude / 7 rounded to
+    `dtype` (1 for a group of zeros, and for one whose scale would round to 0), q the nearest even of weight / scale."""
+    n, k = weight.shape
+    _checked(n, k, group)
+    count = -(-k // group)
+    w = torch.zeros((n, count * group), dtype=torch.float32, device=weight.device)
+    w[:, :k] = weight
+    w = w.view(n, count, group)
+    scales = (w.abs().amax(-1) / 7).to(dtype)
+    scales = torch.where(scales == 0, torch.ones_like(scales), scales)
+    q = torch.round(w / scales.float()[..., None]).clamp_(-8, 7).to(torch.int8)
+    return q.view(n, -1)[:, :k].contiguous(), scales
+
+
+def pack(q: torch.Tensor, scales: torch.Tensor, group: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """q int8 [n, k] in -8 .. 7 and scales [n, ceil(k / group)] -> what the kernel reads (the layout is in tllm_serving_api.h), on the same device."""
+    n, k = q.shape
+    _checked(n, k, group)
+    if q.dtype is not torch.int8 or scales.dtype not in _ACT or tuple(scales.shape) != (n, -(-k // group)) or scales.device != q.device:
+        raise ValueError(f'q has to be int8 [n, k] and the scales float16 or bfloat16 [n, {-(-k // group)}] on one device: got {q.dtype} {tuple(q.shape)}, '
+                         f'{scales.dtype} {tuple(scales.shape)}')
+    if int(q.min()) < -8 or int(q.max()) > 7:
+        raise ValueError('q has values outside -8 .. 7')
+    tiles, steps = -(-n // 16), -(-k // 128)
+    u = torch.full((16 * tiles, 128 * steps), 8, dtype=torch.uint8, device=q.device)
+    u[:n, :k] = (q + 8).to(torch.uint8)
+    u = u.view(tiles, 16, steps, 4, 4, 8)[..., _ORDER]  # [tile, r, k tile, j, g, nibble]
+    u = (u[..., 0::2] | (u[..., 1::2] << 4)).permute(0, 2, 4, 1, 3, 5)  # [tile, k tile, g, r, j, byte]
+    s = torch.zeros((scales.shape[1], 16 * tiles), dtype=scales.dtype, device=q.device)
+    s[:, :n] = scales.t()
+    return u.reshape(tiles, steps, 64, 16).contiguous(), s
+
+
+class GroupQuantMatmul(object):
+    """y = x W^T with W packed once: q int8 [n, k] in -8 .. 7, scales float16 or bfloat16 [n, ceil(k / group)], which is the type of x and y too."""
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor, group: int):
+        self.n, self.k, self.group, self.dtype = q.shape[0], q.shape[1], group, scales.dtype
+        self.packed, self.scales = pack(q, scales, group)
+        if self.packed.device.type != 'cuda':
+            raise ValueError(f'the weights have to be on a GPU: got {self.packed.device}')
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor, group: int, dtype=torch.float16) -> 'GroupQuantMatmul':
+        return cls(*quantize(weight, group, dtype), group)
+
+    def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [.., k] -> [.., n]; a two-dimensional x may have strided rows.  `out` [rows, n] takes the result if given."""
+        if x.dtype is not self.dtype or x.shape[-1] != self.k or x.device != self.packed.device:
+            raise ValueError(f'x has to be {self.dtype} [.., {self.k}] on {self.packed.device}: got {x.dtype} {tuple(x.shape)} on {x.device}')
+        x2 = x if x.dim() == 2 else x.reshape(-1, self.k)
+        if x2.stride(1) != 1:
+            raise ValueError(f'the rows of x have to be contiguous: got strides {x.stride()}')
+        rows = x2.shape[0]
+        y = torch.empty((rows, self.n), dtype=self.dtype, device=x.device) if out is None else out
+        if y.dtype is not self.dtype or tuple(y.shape) != (rows, self.n) or y.stride(1) != 1 or y.device != x.device:
+            raise ValueError(f'out has to be {self.dtype} [{rows}, {self.n}] with contiguous rows on {x.device}: got {y.dtype} {tuple(y.shape)} on {y.device}')
+        p = _Params(rows, self.n, self.k, self.group, _ACT[self.dtype], x2.stride(0) if rows > 1 else self.k, y.stride(0) if rows > 1 else self.n, x2.data_ptr(), self.packed.data_ptr(), self.scales.data_ptr(), y.data_ptr())
+        index, back = x.device.index, torch.cuda.current_device()
+        if index != back:
+            torch.cuda.set_device(index)
+        try:
+            if _entry()(ctypes.addressof(p), torch.cuda.current_stream(index).cuda_stream):
+                raise RuntimeError(f'GroupQuantMatmul: {capi.last_error()}')
+        finally:
+            if index != back:
+                torch.cuda.set_device(back)
+        return y if out is not None or x.dim() == 2 else y.view(*x.shape[:-1], self.n)
