@@ -584,12 +584,19 @@ def test_wrappers_refuse():
         c.attention(torch.zeros(3, 3, 64, dtype=torch.float16, device='cuda'), t, cu, n, 3)
     with pytest.raises(RuntimeError, match='max_new'):
         c.attention(k, t, cu, n, 0)
-    for bad in ((k, t.long(), cu, n), (k, t[:, ::2], cu[:1], n), (k[..., :32], t, cu, n), (k, t, cu, n.float()), (k, t.t(), cu, n)):
+    for bad in ((k, t.long(), cu, n), (k, t[:, ::2], cu[:1], n), (k[..., :32], t, cu, n), (k, t, cu, n.float()), (k, gpu([[0, 1], [2, 3]]).t(), cu, n)):
         with pytest.raises(ValueError):
             c.attention(*bad, max_new=3)
     for bad in (dict(page_size=48), dict(head_size=96), dict(pool=c.pool.float()), dict(scales=c.scales[:2])):
         with pytest.raises(ValueError):
             P.PagedKV8Cache(**{**dict(pool=c.pool, scales=c.scales, page_size=16, head_size=64), **bad})
+    pool = P.DeviceBlockPool(4, 16, 2, 3)
+    out = P.StepPlan(2, 5)
+    for bad in ((gpu([1, 1]).long(), 5, out), (gpu([1]), 5, out), (gpu([1, 1]), 4, out), (gpu([1, 1]).cpu(), 5, out)):
+        with pytest.raises(ValueError):
+            pool.plan(*bad)
+    with pytest.raises(AttributeError):
+        out.slot_map = gpu([1])
     with pytest.raises(RuntimeError, match='page_size'):
         P.plan_step(n, n, gpu([0, 1]), gpu([0, 2]), t, 24, 3)
     f = G.GroupQuantMatmul(torch.zeros(8, 64, dtype=torch.int8, device='cuda'), torch.ones(8, 1, dtype=torch.float16, device='cuda'), 64)

@@ -2,22 +2,19 @@
 
 Next to WeightOnlyQuantMatmul, whose 4-bit weights have one scale for a whole output channel.  y = x W^T, W[n, k] = q[n, k] s[n, k / group]."""
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from ..plugin import capi
+from ..runtime.paged_kv8 import on_device
 
 GROUPS = (32, 64, 128)
 _ACT = {torch.float16: capi.HALF, torch.bfloat16: 7}
 _ORDER = (0, 2, 4, 6, 1, 3, 5, 7)  # element of a word's eight that nibble i holds
 
-_i32, _i64, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
-
-
-class _Params(ctypes.Structure):
-    _fields_ = [(n, _i32) for n in ('rows', 'n', 'k', 'group', 'dtype')] + [('ldx', _i64), ('ldy', _i64)] + [(n, _ptr) for n in ('x', 'packed', 'scales', 'y')]
-
+_PARAMS = struct.Struct('@5i2q4P')  # tllm_group_matmul_params_t
 
 _matmul = None
 
@@ -26,7 +23,7 @@ def _entry():
     global _matmul
     if _matmul is None:
         f = capi.load_library().tllm_group_matmul
-        f.argtypes, f.restype = [_ptr, _ptr], _i32
+        f.argtypes, f.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int32
         _matmul = f
     return _matmul
 
@@ -80,6 +77,7 @@ class GroupQuantMatmul(object):
         self.packed, self.scales = pack(q, scales, group)
         if self.packed.device.type != 'cuda':
             raise ValueError(f'the weights have to be on a GPU: got {self.packed.device}')
+        self._index, self._act, self._at = self.packed.get_device(), _ACT[self.dtype], (self.packed.data_ptr(), self.scales.data_ptr())
 
     @classmethod
     def from_float(cls, weight: torch.Tensor, group: int, dtype=torch.float16) -> 'GroupQuantMatmul':
@@ -87,23 +85,18 @@ class GroupQuantMatmul(object):
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [.., k] -> [.., n]; a two-dimensional x may have strided rows.  `out` [rows, n] takes the result if given."""
-        if x.dtype is not self.dtype or x.shape[-1] != self.k or x.device != self.packed.device:
-            raise ValueError(f'x has to be {self.dtype} [.., {self.k}] on {self.packed.device}: got {x.dtype} {tuple(x.shape)} on {x.device}')
-        x2 = x if x.dim() == 2 else x.reshape(-1, self.k)
-        if x2.stride(1) != 1:
-            raise ValueError(f'the rows of x have to be contiguous: got strides {x.stride()}')
-        rows = x2.shape[0]
-        y = torch.empty((rows, self.n), dtype=self.dtype, device=x.device) if out is None else out
-        if y.dtype is not self.dtype or tuple(y.shape) != (rows, self.n) or y.stride(1) != 1 or y.device != x.device:
-            raise ValueError(f'out has to be {self.dtype} [{rows}, {self.n}] with contiguous rows on {x.device}: got {y.dtype} {tuple(y.shape)} on {y.device}')
-        p = _Params(rows, self.n, self.k, self.group, _ACT[self.dtype], x2.stride(0) if rows > 1 else self.k, y.stride(0) if rows > 1 else self.n, x2.data_ptr(), self.packed.data_ptr(), self.scales.data_ptr(), y.data_ptr())
-        index, back = x.device.index, torch.cuda.current_device()
-        if index != back:
-            torch.cuda.set_device(index)
-        try:
-            if _entry()(ctypes.addressof(p), torch.cuda.current_stream(index).cuda_stream):
-                raise RuntimeError(f'GroupQuantMatmul: {capi.last_error()}')
-        finally:
-            if index != back:
-                torch.cuda.set_device(back)
-        return y if out is not None or x.dim() == 2 else y.view(*x.shape[:-1], self.n)
+        index, n, k = self._index, self.n, self.k
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        (rows, wide), (row, one) = x2.shape, x2.stride()
+        if x.dtype is not self.dtype or wide != k or one != 1 or x.get_device() != index:
+            raise ValueError(f'x has to be {self.dtype} [.., {k}] with contiguous rows on GPU {index}: got {x.dtype} {tuple(x.shape)} with strides {x.stride()} on {x.device}')
+        if out is None:
+            y, y_row = torch.empty((rows, n), dtype=self.dtype, device=x.device), n
+        else:
+            y, y_row = out, out.stride(0) if rows > 1 else n
+            if y.dtype is not self.dtype or tuple(y.shape) != (rows, n) or (y.stride(1) != 1 and n > 1) or y.get_device() != index:
+                raise ValueError(f'out has to be {self.dtype} [{rows}, {n}] with contiguous rows on GPU {index}: got {y.dtype} {tuple(y.shape)} with strides {y.stride()} on {y.device}')
+        p = _PARAMS.pack(rows, n, k, self.group, self._act, row if rows > 1 else k, y_row, x2.data_ptr(), *self._at, y.data_ptr())
+        if on_device(index, _matmul or _entry(), p):
+            raise RuntimeError(f'GroupQuantMatmul: {capi.last_error()}')
+        return y if out is not None or x.dim() == 2 else y.view(*x.shape[:-1], n)
