@@ -65,68 +65,361 @@ __device__ __forceinline__ float to_f32(uint32_t bits16)
         return h2f((uint16_t) bits16);
 }
 
-// 16 outputs x 16 rows a workgroup, its waves take the k-tiles in turn
-template <bool BF16, int GROUP>
-__global__ __launch_bounds__(256) void rows16_kernel(const tllm_group_matmul_params_t p)
+__device__ __forceinline__ u32x4 as_u32x4(const uint4& v)
 {
-    __shared__ f32x4 part[4][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int n_tile = blockIdx.x, m = blockIdx.y * 16 + r, k_tiles = (p.k + 127) / 128, n_all = (p.n + 15) / 16 * 16;
-    const uint4* const packed = static_cast<const uint4*>(p.packed) + (int64_t) n_tile * k_tiles * 64 + lane;
-    const uint16_t* const scales = static_cast<const uint16_t*>(p.scales) + n_tile * 16 + 4 * g;
-    const uint16_t* const x = static_cast<const uint16_t*>(p.x) + (int64_t) min(m, p.rows - 1) * p.ldx + 8 * g;
-    constexpr int kSteps = GROUP / 32;
-    const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    for (int t = wave; t < k_tiles; t += 4)
-    {
-        const uint4 w4 = packed[t * 64];
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        f32x4 acc, sum;
+    return u32x4{v.x, v.y, v.z, v.w};
+}
+
+// y += s * (acc - what the raw bfloat16 weights count too much)
+template <bool BF16>
+__device__ __forceinline__ void scaled_add(f32x4& y, const f32x4& acc, const f32x4& sum, uint2 s)
+{
+    const float f[4] = {to_f32<BF16>(s.x & 0xffffu), to_f32<BF16>(s.x >> 16), to_f32<BF16>(s.y & 0xffffu), to_f32<BF16>(s.y >> 16)};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-        {
-            const int k = t * 128 + j * 32;
-            if (k >= p.k)
-                break;
-            const uint4 x4 = *reinterpret_cast<const uint4*>(x + k);
-            const u32x4 b = {x4.x, x4.y, x4.z, x4.w};
-            if (j % kSteps == 0)
-                acc = sum = f32x4{0.f, 0.f, 0.f, 0.f};
-            acc = product<BF16>(weights8<BF16>(w[j]), b, acc);
-            if (BF16)
-                sum = product<BF16>(ones, b, sum);
-            if (j % kSteps == kSteps - 1 || k + 32 >= p.k)
-            {
-                const uint2 s = *reinterpret_cast<const uint2*>(scales + (int64_t) (k / GROUP) * n_all);
-                if (BF16)
-                    acc -= 136.f * sum;
-                y[0] += to_f32<BF16>(s.x & 0xffffu) * acc[0];
-                y[1] += to_f32<BF16>(s.x >> 16) * acc[1];
-                y[2] += to_f32<BF16>(s.y & 0xffffu) * acc[2];
-                y[3] += to_f32<BF16>(s.y >> 16) * acc[3];
-            }
-        }
-    }
-    part[wave][lane] = y;
-    __syncthreads();
-    if (wave != 0 || m >= p.rows)
-        return;
-    y = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+    for (int i = 0; i < 4; ++i)
+        y[i] += f[i] * (BF16 ? acc[i] - 136.f * sum[i] : acc[i]);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store4(const tllm_group_matmul_params_t& p, const f32x4& y, int m, int n)
+{
     uint16_t* const to = static_cast<uint16_t*>(p.y) + (int64_t) m * p.ldy;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
+        if (n + i < p.n)
+            to[n + i] = BF16 ? f2bf(y[i]) : f2h(y[i]);
+}
+
+__device__ const uint4 kZeros[1] = {};
+
+// 64 lanes x 16 bytes to LDS, lane by lane from lds_byte on; what is under way is counted by hand
+__device__ __forceinline__ void dma16(const void* from, uint32_t lds_byte)
+{
+    uint32_t m0_keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(m0_keep) : "v"(from), "s"(lds_byte) : "memory");
+}
+
+// Up to 4 R rows: a workgroup has 16 NT outputs, its waves share the k-tiles out and join through LDS.  What it has to read is the weights, once;
+// each CU also reads all of x, which is as much as its weights at 8 rows and 16 outputs and is why x comes by whole 256-byte pieces of the
+// rows that there are.  A wave has a ring of DEEP k-tiles in LDS, its own: no barrier, only the count of what is under way.
+template <int R, int NT>
+struct FewForm
+{
+    static constexpr int kSlot = R + NT + 1; // KB: x, weights, scales
+    static constexpr int kWaves = kSlot <= 4 ? 16 : kSlot <= 9 ? 8 : 4, kFit = 152 / (kWaves * kSlot), kDeep = kFit < 4 ? kFit : 4;
+    static constexpr int kRing = kWaves * kDeep * kSlot * 1024, kMT = (R + 3) / 4;
+    static_assert(kDeep >= 1 && kWaves * kMT * NT * 1024 <= 160 * 1024 && (kDeep - 1) * kSlot < 64, "the ring fits LDS and the counter");
+    static constexpr int kLds = kRing > kWaves * kMT * NT * 1024 ? kRing : kWaves * kMT * NT * 1024;
+};
+
+template <bool BF16, int GROUP, int R, int NT>
+__global__ __launch_bounds__((64 * FewForm<R, NT>::kWaves)) void few_rows_kernel(const tllm_group_matmul_params_t p)
+{
+    using F = FewForm<R, NT>;
+    constexpr int kSteps = GROUP / 32, kGroups = 4 / kSteps, MT = F::kMT, kMask = R < 4 ? 4 * R - 1 : 15;
+    extern __shared__ uint4 lds[];
+    typedef __attribute__((address_space(3))) void lds_t;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int k_tiles = (p.k + 127) / 128, n_tiles = (p.n + 15) / 16, n_all = n_tiles * 16, n0 = blockIdx.x * NT;
+    const int groups = (p.k + GROUP - 1) / GROUP;
+    const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t lds0 = (uint32_t) (uintptr_t) (lds_t*) lds + wave * F::kDeep * F::kSlot * 1024;
+
+    auto bring = [&](int slot, int t) {
+        const uint32_t to = lds0 + slot * F::kSlot * 1024;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+        {
+            // rows of 256 bytes, piece c of 16 bytes at c ^ row: the 16 rows of a fragment read 16 different places
+            const int row = 4 * i + g, k = t * 128 + ((r ^ (row & 15)) << 3);
+            const void* from = static_cast<const uint16_t*>(p.x) + (int64_t) min(row, p.rows - 1) * p.ldx + k;
+            dma16(k < p.k ? from : static_cast<const void*>(kZeros), to + i * 1024);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) // a tile behind the last one is computed again and not written
+            dma16(static_cast<const uint4*>(p.packed) + ((int64_t) min(n0 + i, n_tiles - 1) * k_tiles + t) * 64 + lane, to + (R + i) * 1024);
+        const int piece = min(lane, 2 * NT * kGroups - 1), q = piece / (2 * NT), n = n0 * 16 + (piece - q * 2 * NT) * 8;
+        dma16(static_cast<const uint16_t*>(p.scales) + (int64_t) min(t * kGroups + q, groups - 1) * n_all + min(n, n_all - 8), to + (R + NT) * 1024);
+    };
+    f32x4 y[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+            y[i][j] = zero;
+#pragma unroll
+    for (int d = 0; d < F::kDeep; ++d)
+        if (wave + d * F::kWaves < k_tiles)
+            bring(d, wave + d * F::kWaves);
+    int slot = 0;
+    for (int t = wave; t < k_tiles; t += F::kWaves)
     {
-        const int n = n_tile * 16 + 4 * g + i;
-        if (n < p.n)
-            to[n] = BF16 ? f2bf(y[i]) : f2h(y[i]);
+        if (t + (F::kDeep - 1) * F::kWaves < k_tiles)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((F::kDeep - 1) * F::kSlot) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const uint4* const at = lds + (wave * F::kDeep + slot) * F::kSlot * 64;
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q)
+        {
+            u32x4 b[kSteps][MT];
+            f32x4 sum[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+            {
+                sum[i] = zero;
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j)
+                {
+                    const int row = r & kMask;
+                    b[j][i] = as_u32x4(at[(16 * i + row) * 16 + ((4 * (q * kSteps + j) + g) ^ row)]);
+                    if (BF16)
+                        sum[i] = product<BF16>(ones, b[j][i], sum[i]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+            {
+                const uint32_t* const words = reinterpret_cast<const uint32_t*>(at + (R + n) * 64 + lane) + q * kSteps;
+                const uint2 s = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(at + (R + NT) * 64) + (q * NT + n) * 16 + 4 * g);
+                f32x4 acc[MT];
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j)
+                {
+                    const u32x4 a = weights8<BF16>(words[j]);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        acc[i] = product<BF16>(a, b[j][i], j ? acc[i] : zero);
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    scaled_add<BF16>(y[n][i], acc[i], sum[i], s);
+            }
+        }
+        if (t + F::kDeep * F::kWaves < k_tiles)
+        {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the slot is read
+            bring(slot, t + F::kDeep * F::kWaves);
+        }
+        slot = slot + 1 == F::kDeep ? 0 : slot + 1;
     }
+    __syncthreads(); // every wave is through with its ring: it takes the sums now
+    f32x4* const part = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+            part[(wave * NT * MT + i * MT + j) * 64 + lane] = y[i][j];
+    __syncthreads();
+    for (int u = wave; u < NT * MT; u += F::kWaves)
+    {
+        f32x4 v = part[u * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < F::kWaves; ++w)
+            v += part[(w * NT * MT + u) * 64 + lane];
+        const int n = (n0 + u / MT) * 16 + 4 * g, m = u % MT * 16 + r;
+        if (m < p.rows)
+            store4<BF16>(p, v, m, n);
+    }
+}
+
+// Many rows: 128 rows x 64 NT outputs a workgroup of 8 waves, 64 x 16 NT a wave.  x, weights and scales of a k-tile go to LDS by DMA, x and weights as the
+// fragments that the waves read back (64 lanes x 16 bytes in a row: no conflicts), three k-tiles in a ring: two are under way while one is
+// multiplied.  One barrier a k-tile: behind it the tile before is free and the next but one is sent for.
+constexpr int kStages = 3;
+
+template <int GROUP, int NT>
+struct TileForm
+{
+    static constexpr int kGroups = 128 / GROUP, kOutTiles = 4 * NT; // tiles of 16 outputs
+    static constexpr int kX = 32, kW = kOutTiles, kChunks = kX + kW + kGroups, kPerWave = (kChunks + 7) / 8; // of 1 KB, per k-tile
+    static constexpr int kStageBytes = kChunks * 1024;
+};
+
+template <bool BF16, int GROUP, int NT>
+__global__ __launch_bounds__(512, 2) void tile_kernel(const tllm_group_matmul_params_t p, const int m_tiles, const int tiles)
+{
+    using F = TileForm<GROUP, NT>;
+    constexpr int kSteps = GROUP / 32;
+    extern __shared__ uint4 lds[]; // [kStages]: x [8 row tiles][4][64], weights [kOutTiles][64], scales [kGroups][64]
+    typedef __attribute__((address_space(3))) void lds_t;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    // workgroups go round the XCDs: each XCD takes a contiguous range of the tiles, whose row tiles share their weights in its L2
+    const int q8 = tiles >> 3, r8 = tiles & 7, xcd = blockIdx.x & 7;
+    const int id = xcd * q8 + min(xcd, r8) + (blockIdx.x >> 3);
+    const int tile_n = id / m_tiles, tile_m = id - tile_n * m_tiles;
+    const int k_tiles = (p.k + 127) / 128, n_tiles = (p.n + 15) / 16, n_all = n_tiles * 16, groups = (p.k + GROUP - 1) / GROUP;
+    const int wn = wave & 3, wm = wave >> 2, n0 = tile_n * F::kOutTiles;
+    const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t lds0 = (uint32_t) (uintptr_t) (lds_t*) lds;
+
+    // chunk c of a k-tile: x (row tile c / 4, k-step c % 4), then weights, then scales; a wave brings chunks wave, wave + 8, .. (the last one once
+    // more where they do not divide)
+    auto bring = [&](int t) {
+        const uint32_t to = lds0 + (t % kStages) * F::kStageBytes;
+#pragma unroll
+        for (int i = 0; i < F::kPerWave; ++i)
+        {
+            const int c = min(i * 8 + wave, F::kChunks - 1);
+            const void* from;
+            if (c < F::kX)
+            {
+                const int k = t * 128 + 32 * (c & 3) + 8 * g;
+                from = static_cast<const uint16_t*>(p.x) + (int64_t) min((tile_m * 8 + (c >> 2)) * 16 + r, p.rows - 1) * p.ldx + k;
+                from = k < p.k ? from : static_cast<const void*>(kZeros);
+            }
+            else if (c < F::kX + F::kW)
+                from = static_cast<const uint4*>(p.packed) + ((int64_t) min(n0 + c - F::kX, n_tiles - 1) * k_tiles + t) * 64 + lane;
+            else
+                from = static_cast<const uint16_t*>(p.scales) + (int64_t) min(t * F::kGroups + c - F::kX - F::kW, groups - 1) * n_all + min(n0 * 16 + lane * 8, n_all - 8);
+            dma16(from, to + c * 1024);
+        }
+    };
+    f32x4 y[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            y[i][j] = zero;
+
+    bring(0);
+    if (k_tiles > 1)
+        bring(1);
+    for (int t = 0; t < k_tiles; ++t)
+    {
+        // this k-tile has arrived (the next may be under way), for every wave, and the one before is read
+        if (t + 1 < k_tiles)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(F::kPerWave) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t + 2 < k_tiles)
+            bring(t + 2);
+        const uint4* const at = lds + (t % kStages) * (F::kStageBytes / 16);
+        const uint4* const xs = at + wm * 4 * 4 * 64 + lane;
+        const uint4* const ws = at + (F::kX + wn * NT) * 64 + lane;
+        const char* const ss = reinterpret_cast<const char*>(at + (F::kX + F::kW) * 64) + (wn * NT * 16 + 4 * g) * 2;
+#pragma unroll
+        for (int q = 0; q < F::kGroups; ++q)
+        {
+            u32x4 b[kSteps][4];
+            f32x4 sum[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j)
+                    b[j][i] = as_u32x4(xs[(i * 4 + q * kSteps + j) * 64]);
+                if (BF16)
+                {
+                    sum[i] = zero;
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j)
+                        sum[i] = product<BF16>(ones, b[j][i], sum[i]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+            {
+                const uint32_t* const words = reinterpret_cast<const uint32_t*>(ws + n * 64) + q * kSteps;
+                const uint2 s = *reinterpret_cast<const uint2*>(ss + q * 1024 + n * 32);
+                f32x4 acc[4];
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j)
+                {
+                    const u32x4 a = weights8<BF16>(words[j]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[i] = product<BF16>(a, b[j][i], j ? acc[i] : zero);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    scaled_add<BF16>(y[n][i], acc[i], sum[i], s);
+            }
+        }
+    }
+    const bool whole = p.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        const int m = (tile_m * 8 + wm * 4 + i) * 16 + r;
+        if (m >= p.rows)
+            continue;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+        {
+            const int n = (n0 + wn * NT + j) * 16 + 4 * g;
+            const f32x4 v = y[j][i];
+            if (whole && n + 4 <= p.n)
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + (int64_t) m * p.ldy + n)
+                    = BF16 ? make_uint2((uint32_t) f2bf(v[0]) | (uint32_t) f2bf(v[1]) << 16, (uint32_t) f2bf(v[2]) | (uint32_t) f2bf(v[3]) << 16)
+                           : make_uint2((uint32_t) f2h(v[0]) | (uint32_t) f2h(v[1]) << 16, (uint32_t) f2h(v[2]) | (uint32_t) f2h(v[3]) << 16);
+            else if (n < p.n)
+                store4<BF16>(p, v, m, n);
+        }
+    }
+}
+
+template <bool BF16, int GROUP, int NT>
+void launch_tiles(const tllm_group_matmul_params_t& p, int m_tiles, int n_parts, hipStream_t stream)
+{
+    const size_t lds = kStages * TileForm<GROUP, NT>::kStageBytes;
+    launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&tile_kernel<BF16, GROUP, NT>), lds);
+    tile_kernel<BF16, GROUP, NT><<<m_tiles * n_parts, 512, lds, stream>>>(p, m_tiles, m_tiles * n_parts);
+}
+
+// 256 or 192 outputs a workgroup, one workgroup a CU: whichever gets by with less work in its rounds
+template <bool BF16, int GROUP>
+void launch_many(const tllm_group_matmul_params_t& p, hipStream_t stream)
+{
+    const int cus = launch_util::device_cus(), m_tiles = (p.rows + 127) / 128, n4 = (p.n + 255) / 256, n3 = (p.n + 191) / 192;
+    const int64_t rounds4 = ((int64_t) m_tiles * n4 + cus - 1) / cus, rounds3 = ((int64_t) m_tiles * n3 + cus - 1) / cus;
+    if (rounds3 * 3 < rounds4 * 4)
+        launch_tiles<BF16, GROUP, 3>(p, m_tiles, n3, stream);
+    else
+        launch_tiles<BF16, GROUP, 4>(p, m_tiles, n4, stream);
+}
+
+template <bool BF16, int GROUP, int R, int NT>
+void launch_few(const tllm_group_matmul_params_t& p, hipStream_t stream)
+{
+    using F = FewForm<R, NT>;
+    launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&few_rows_kernel<BF16, GROUP, R, NT>), F::kLds);
+    few_rows_kernel<BF16, GROUP, R, NT><<<((p.n + 15) / 16 + NT - 1) / NT, 64 * F::kWaves, F::kLds, stream>>>(p);
+}
+
+// as few outputs a workgroup as give one workgroup a CU (a CU reads x once then), at most 64
+template <bool BF16, int GROUP, int R>
+void launch_rows(const tllm_group_matmul_params_t& p, hipStream_t stream)
+{
+    const int cus = launch_util::device_cus(), n_tiles = (p.n + 15) / 16;
+    if (n_tiles <= cus)
+        launch_few<BF16, GROUP, R, 1>(p, stream);
+    else if (n_tiles <= 2 * cus)
+        launch_few<BF16, GROUP, R, 2>(p, stream);
+    else if (n_tiles <= 3 * cus)
+        launch_few<BF16, GROUP, R, 3>(p, stream);
+    else
+        launch_few<BF16, GROUP, R, 4>(p, stream);
 }
 
 template <bool BF16, int GROUP>
 void launch_form(const tllm_group_matmul_params_t& p, hipStream_t stream)
 {
-    rows16_kernel<BF16, GROUP><<<dim3((p.n + 15) / 16, (p.rows + 15) / 16), 256, 0, stream>>>(p);
+    if (p.rows <= 4)
+        launch_rows<BF16, GROUP, 1>(p, stream);
+    else if (p.rows <= 8)
+        launch_rows<BF16, GROUP, 2>(p, stream);
+    else if (p.rows <= 16)
+        launch_rows<BF16, GROUP, 4>(p, stream);
+    else if (p.rows <= 32)
+        launch_rows<BF16, GROUP, 8>(p, stream);
+    else if (p.rows <= 64)
+        launch_rows<BF16, GROUP, 16>(p, stream);
+    else
+        launch_many<BF16, GROUP>(p, stream);
 }
 } // namespace
 
