@@ -101,7 +101,7 @@ int32_t tllm_paged_append(const tllm_paged_append_params_t* p, tllm_stream_t str
  * cu_tokens[b + 1] of q and out and kv_lens[b] cached tokens, its own rows' keys the last of them: its i-th of n rows is the token at
  * kv_lens[b] - n + i and sees the keys up to itself, the last `window` of them if window > 0.  A row that sees none (a length shorter than its
  * rows) is 0.  Query head h reads key head h / (q_heads / kv_heads).  Rows that belong to no request stay as they were.
- * Scores, softmax and sums in fp32; the weights enter the second product as fp16 (rounding 2^-11), bfloat16 queries as fp16 under a power of two
+ * scale >= 0.  Scores, softmax and sums in fp32; the weights enter the second product as fp16 (rounding 2^-11), bfloat16 queries as fp16 under a power of two
  * per row (exact down to 2^-24 of the row's largest).
  *   max_new  no request has more rows (rows behind that many are not computed);
  *   max_kv   an expectation of the longest kv_lens, for how the work is split; any kv_lens up to max_blocks * page_size is right.

@@ -1,22 +1,25 @@
 // Attention over the 8-bit cache with a scale for each page and head (tllm_paged_attention).
 //
-// rows_kernel: one workgroup per (request, key head, 16 rows, part of the keys).  The rows of a key head are its query heads of one token,
-// then those of the next, so that a decoded token of grouped heads is one tile.  Four waves take tiles of 64 keys in turn; each runs the
-// one-pass softmax (running maximum m and sum l, O rescaled when m grows) and they join through LDS.
+// The rows of a key head are its query heads of one token, then those of the next, so that a decoded token of grouped heads is one tile of 16 rows.
+// Both kernels run the one-pass softmax (running maximum m and sum l, O rescaled when m grows) over tiles of 64 keys:
 //   S^T = K Q^T by v_mfma_f32_16x16x32_f16, O^T += V^T P^T by the same.  Which key an MFMA row stands for, and which dimension or key a
-//   k-element, is free as long as both operands agree, so it is chosen for the cache's bytes: lane l = 16 g + r of tile t takes key
-//   16 (r / 4) + 4 t + r % 4, whose scores come back to the lanes of group g = r / 4 of the result, 16 consecutive keys a lane; of a
-//   key a lane takes dimensions 64 j + 16 g .. + 15 (two k-steps).  Every load is 16 bytes of a row of keys or of a channel of values,
-//   no operand passes through LDS, and P goes from the first product's registers into the second's as it is.
-//   16 keys lie in one page, so a lane has one key scale and one value scale per tile.
-// 8-bit elements become fp16 exactly (int8: 0x6400 | (q + 128) = 1152 + q; e4m3: the convert instruction); scales enter in fp32: the key's with the
-// softmax scale behind the first product, the value's into P relative to the largest value scale so far, times 2^15 (P <= 1 and the
-// ratio <= 1: nothing overflows, and nothing is lost until a page's scale is 2^-29 of another's).
-// Few rows and long contexts: the keys are also split over workgroups, the parts joined by merge_kernel in fp32.
+//   k-element, is free as long as both operands agree, so it is chosen for the cache's bytes: lane l = 16 g + r of part i takes key
+//   16 (r / 4) + 4 i + r % 4, whose scores come back to the lanes of group g = r / 4 of the result, 16 consecutive keys a lane; of a
+//   key a lane takes dimensions 64 j + 16 g .. + 15 (two k-steps).  Every load is 16 bytes of a row of keys or of a channel of values, and
+//   P goes from the first product's registers into the second's as it is.  16 keys lie in one page, so a lane has one key scale and one value
+//   scale per tile.
+// 8-bit elements become fp16 exactly (int8: 0x6400 | (q + 128) = 1152 + q; e4m3: the convert instruction).  Scales enter in fp32: the key's with the
+// softmax scale behind the first product; the value's, relative to the largest value scale so far and times 2^15, in the exponent of the
+// weight (P <= 2^15: nothing overflows, and a weight keeps its 11 bits until its page's scale is 2^-29 of another's).
+//   rows_body   16 rows: four or eight waves take tiles in turn, straight from memory into registers, and join through LDS.  Single tokens are bound by
+//               the cache's bytes; the keys are also split over workgroups, whose parts merge_kernel joins.
+//   tile_kernel 64 or 128 rows: the waves share the tiles, which they bring to LDS as fp16 fragments, the next one while this one is computed.  Prompts
+//               are bound by the arithmetic: products, exponentials, and the conversions, which are once a workgroup here and not once a wave.
 #include "dev_utils.h"
 #include "launch_util.h"
 #include "serving_kernels.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace tllm
 {
@@ -32,8 +35,12 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kPScale = 32768.f; // 2^15, see above
+constexpr float kPShift = 15.f; // see above
 constexpr int kTile = 64;
+#ifndef PARTS_WANT
+#define PARTS_WANT 8
+#define PARTS_KEYS 256
+#endif
 
 __device__ __forceinline__ f16x8 join(u32x4 w)
 {
@@ -167,58 +174,158 @@ struct Split
     int parts;
 };
 
-template <int DIM, bool BF16, bool FP8>
-__global__ __launch_bounds__(256) void rows_kernel(const tllm_paged_attention_params_t p, const int shift, const int row_tiles, const Split split)
+// What a tile's pages say to a lane: their scales, and how its weights are scaled for the second product.
+struct TileScales
 {
-    constexpr int kSteps = DIM / 32, kOut = DIM / 16, kLine = DIM + 4;
-    __shared__ float acc[2][16][kLine];
-    __shared__ float ms[4][16], ls[4][16];
+    float ks, vs;
+    float lift, drop; // weights are formed times 2^lift; 2^-lift
+    float back;       // what O has to be multiplied by as the reference grows
+};
+__device__ __forceinline__ TileScales scales_of(float ks, float vs, float& v_ref)
+{
+    TileScales t;
+    t.ks = ks;
+    t.vs = vs;
+    const float v_new = fmaxf(v_ref, groups_max(vs));
+    t.back = v_new > v_ref ? v_ref / v_new : 1.f;
+    // below 2^-60 of the reference a page's weights are 0 in fp16 either way; l still has to see them
+    t.lift = v_new > 0.f ? fmaxf(__builtin_amdgcn_logf(vs / v_new) + kPShift, -60.f) : 0.f;
+    t.drop = __builtin_amdgcn_exp2f(-t.lift);
+    v_ref = v_new;
+    return t;
+}
+
+// One tile of one row: the 16 scores of a lane (keys key0 .. + 15 of a query's row) -> its weights in fp16, with m, l and O brought along.  `plain`
+// (the same for the wave): every key is seen.
+template <int N>
+__device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], float& m, float& l, f32x4 (&o)[N], const TileScales& t, float factor, bool plain, bool in, int key0,
+    int from, int seen)
+{
+    float f = factor * t.ks;
+    if (!plain)
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            s[i] = in && key0 + i < seen && key0 + i >= from ? s[i] * f : -INFINITY;
+        f = 1.f;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i)
+        top = fmaxf(top, s[i]);
+    const float m_new = fmaxf(m, groups_max(top * f)), m_use = m_new == -INFINITY ? 0.f : m_new; // f >= 0
+    if (__builtin_amdgcn_ballot_w64(m_new != m || t.back != 1.f))
+    {
+        const float alpha = __builtin_amdgcn_exp2f(m - m_use), back = alpha * t.back;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            o[i] *= back;
+    }
+    m = m_new;
+    const float shift = t.lift - m_use;
+    float sum = 0.f;
+    u32x4 p[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], f, shift)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], f, shift));
+        sum += a + b;
+        p[i >> 2][i & 3] = pack_f16(a, b);
+    }
+    l += sum * t.drop;
+    w[0] = join(p[0]);
+    w[1] = join(p[1]);
+}
+
+template <int DIM>
+struct RowsLds
+{
+    static constexpr int kLine = DIM + 4;
+    static constexpr int bytes(int nw) { return (nw / 2 * 16 * kLine + nw * 32) * 4; }
+};
+
+// 16 rows (`tile`) of a request and key head, keys of one part: NW waves
+template <int DIM, bool BF16, bool FP8, int NW>
+__device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p, const int shift, const Split& split, const Request& req, int head, int b, int tile, int part,
+    float* lds)
+{
+    constexpr int kSteps = DIM / 32, kOut = DIM / 16, kLine = RowsLds<DIM>::kLine, kPlaces = NW / 2;
+    float(*acc)[16][kLine] = reinterpret_cast<float(*)[16][kLine]>(lds);
+    float(*ms)[16] = reinterpret_cast<float(*)[16]>(lds + kPlaces * 16 * kLine);
+    float(*ls)[16] = ms + NW;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
-    int id = blockIdx.x;
-    const int part = id % split.parts;
-    id /= split.parts;
-    const int tile = id % row_tiles;
-    id /= row_tiles;
-    const int head = id % p.kv_heads, b = id / p.kv_heads, group = p.q_heads / p.kv_heads;
-    const Request req = request_of(p, b, shift);
+    const int group = p.q_heads / p.kv_heads;
     const int rows = min(req.rows, p.max_new) * group, row = tile * 16 + r;
-    if (tile * 16 >= rows)
-        return;
     const int first = req.len - req.rows; // position of the request's first row
     const bool live = row < rows;
     const int token = row / group, qh = head * group + row - token * group;
-    const int seen = live ? first + token + 1 : 0; // keys [from, seen) are visible to the lane's row
-    const int from = p.window > 0 ? seen - p.window : 0;
+    const int seen = live ? first + token + 1 : 0x7fffffff; // keys [from, seen) are visible to the lane's row; a row that is none masks nothing
+    const int from = live && p.window > 0 ? seen - p.window : 0;
     const int last = min(tile * 16 + 15, rows - 1) / group;
     const int lo = p.window > 0 ? max(0, first + tile * 16 / group + 1 - p.window) : 0, hi = first + last + 1;
     const int t_lo = lo / kTile, n_tiles = max(0, (hi + kTile - 1) / kTile - t_lo), per = (n_tiles + split.parts - 1) / split.parts;
     const int t_begin = t_lo + min(n_tiles, part * per), t_end = t_lo + min(n_tiles, (part + 1) * per);
-
-    f16x8 q[kSteps];
-    const uint16_t* const q_row = live ? static_cast<const uint16_t*>(p.q) + (req.row0 + token) * p.q_row + qh * p.q_head : nullptr;
-    const float factor = load_query<DIM, BF16>(q, q_row, g) * p.scale * kLog2e;
 
     const int page = 1 << shift;
     const int64_t head_bytes = (int64_t) page * DIM, side_bytes = head_bytes * p.kv_heads;
     const uint8_t* const pool = static_cast<const uint8_t*>(p.pool) + head * head_bytes;
     const int32_t* const table = p.block_table + (int64_t) b * p.table_stride;
 
+    // What a tile needs of memory, each part sent for as soon as its registers are free: blocks two tiles ahead, keys and scales behind the
+    // first product, values behind the second.
+    int kb = -1, vb = -1; // blocks of the lane's 16 keys in the first and the second product, -1: none
+    u32x4 kw[4][DIM / 64], vw[kOut];
+    float ks_next = 0.f, vs_next = 0.f;
+    auto blocks_of = [&](int t) {
+        const int kk = t * kTile + 16 * (r >> 2), vk = t * kTile + 16 * g;
+        kb = kk < req.len ? table[kk >> shift] : -1;
+        vb = vk < req.len ? table[vk >> shift] : -1;
+    };
+    auto held = [&](int block) { return (uint32_t) block < (uint32_t) p.num_blocks; };
+    auto fetch_keys = [&](int t) {
+        const uint8_t* const at = pool + (int64_t) (held(kb) ? kb : 0) * 2 * side_bytes + (((t * kTile + 16 * (r >> 2)) & (page - 1)) + (r & 3)) * DIM + 16 * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < DIM / 64; ++j)
+                kw[i][j] = *reinterpret_cast<const u32x4*>(at + 4 * i * DIM + 64 * j);
+        const float* const s_at = p.scales + (int64_t) (held(vb) ? vb : 0) * 2 * p.kv_heads + head;
+        ks_next = s_at[0];
+        vs_next = s_at[p.kv_heads];
+    };
+    auto fetch_values = [&](int t, int block) {
+        const uint8_t* const at = pool + ((int64_t) (held(block) ? block : 0) * 2 + 1) * side_bytes + r * page + ((t * kTile + 16 * g) & (page - 1));
+#pragma unroll
+        for (int i = 0; i < kOut; ++i)
+            vw[i] = *reinterpret_cast<const u32x4*>(at + 16 * i * page);
+    };
+    const int t0 = t_begin + wave;
+    int vb_now = -1;
+    if (t0 < t_end)
+    {
+        blocks_of(t0);
+        vb_now = vb;
+        fetch_keys(t0);
+        fetch_values(t0, vb_now);
+        if (t0 + NW < t_end)
+            blocks_of(t0 + NW);
+    }
+    f16x8 q[kSteps];
+    const uint16_t* const q_row = live ? static_cast<const uint16_t*>(p.q) + (req.row0 + token) * p.q_row + qh * p.q_head : nullptr;
+    const float factor = load_query<DIM, BF16>(q, q_row, g) * p.scale * kLog2e;
+
     f32x4 o[kOut];
 #pragma unroll
     for (int i = 0; i < kOut; ++i)
         o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f, v_ref = 0.f;
-    for (int t = t_begin + wave; t < t_end; t += 4)
-    {
-        const int key0 = t * kTile;
-        const int kk = key0 + 16 * (r >> 2), vk = key0 + 16 * g; // first keys of the lane's 16 in the first and the second product
-        const int kb = kk < req.len ? table[kk >> shift] : -1, vb = vk < req.len ? table[vk >> shift] : -1;
-        const bool k_in = (uint32_t) kb < (uint32_t) p.num_blocks, v_in = (uint32_t) vb < (uint32_t) p.num_blocks;
-        const uint8_t* const k_at = pool + (int64_t) (k_in ? kb : 0) * 2 * side_bytes + ((kk & (page - 1)) + (r & 3)) * DIM + 16 * g;
-        const uint8_t* const v_at = pool + ((int64_t) (v_in ? vb : 0) * 2 + 1) * side_bytes + r * page + (vk & (page - 1));
-        const float* const s_at = p.scales + (int64_t) (v_in ? vb : 0) * 2 * p.kv_heads + head;
-        const float ks = v_in ? s_at[0] : 0.f, vs = v_in ? s_at[p.kv_heads] : 0.f;
-
+    // The last tile of a wave sends for nothing.  It is a body of its own: with the loads under a condition inside one loop the compiler's scheduler
+    // has written over registers of the values that were still to be read (hipcc 7.2, seen in the assembly and by the tests).
+    auto step = [&](int t, auto more) {
+        const int vk = t * kTile + 16 * g;
+        const bool v_in = held(vb_now);
+        const float ks = v_in ? ks_next : 0.f, vs = v_in ? vs_next : 0.f;
         float s[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -227,57 +334,44 @@ __global__ __launch_bounds__(256) void rows_kernel(const tllm_paged_attention_pa
 #pragma unroll
             for (int j = 0; j < DIM / 64; ++j)
             {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(k_at + 4 * i * DIM + 64 * j);
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight<FP8>(w[0], w[1]), q[2 * j], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight<FP8>(w[2], w[3]), q[2 * j + 1], c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight<FP8>(kw[i][j][0], kw[i][j][1]), q[2 * j], c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight<FP8>(kw[i][j][2], kw[i][j][3]), q[2 * j + 1], c, 0, 0, 0);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 s[4 * i + e] = c[e];
         }
-        const float f = factor * ks;
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
+        const int vb_next = vb;
+        if constexpr (more)
         {
-            const int key = vk + i;
-            s[i] = v_in && key < seen && key >= from ? s[i] * f : -INFINITY;
-            top = fmaxf(top, s[i]);
+            fetch_keys(t + NW);
+            if (t + 2 * NW < t_end)
+                blocks_of(t + 2 * NW);
         }
-        const float m_new = fmaxf(m, groups_max(top)), m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float v_new = fmaxf(v_ref, groups_max(vs));
-        const float alpha = __builtin_amdgcn_exp2f(m - m_use);
-        if (__builtin_amdgcn_ballot_w64(m_new != m || v_new != v_ref))
-        {
-            const float back = alpha * (v_new > 0.f ? v_ref / v_new : 1.f);
-            l *= alpha;
+        const TileScales scales = scales_of(ks, vs, v_ref);
+        const int keep = v_in ? req.len - vk : 0;
+        f16x8 w[2];
+        soften(s, w, m, l, o, scales, factor, __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen || vk < from) == 0, v_in, vk, from, seen);
+        if (__builtin_amdgcn_ballot_w64(keep < 16))
 #pragma unroll
             for (int i = 0; i < kOut; ++i)
-                o[i] *= back;
-        }
-        m = m_new;
-        v_ref = v_new;
-        const float up = v_new > 0.f ? vs / v_new * kPScale : 0.f;
-        u32x4 w[2];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-        {
-            const float a = __builtin_amdgcn_exp2f(s[2 * i] - m_use), c = __builtin_amdgcn_exp2f(s[2 * i + 1] - m_use);
-            l += a + c;
-            w[i >> 2][i & 3] = pack_f16(a * up, c * up);
-        }
-        const f16x8 p0 = join(w[0]), p1 = join(w[1]);
-        const int keep = v_in ? req.len - vk : 0;
-        const bool whole = __builtin_amdgcn_ballot_w64(keep < 16) == 0;
+                vw[i] = cut(vw[i], keep);
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
         {
-            u32x4 v = *reinterpret_cast<const u32x4*>(v_at + 16 * i * page);
-            if (!whole)
-                v = cut(v, keep);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight<FP8>(v[0], v[1]), p0, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight<FP8>(v[2], v[3]), p1, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight<FP8>(vw[i][0], vw[i][1]), w[0], o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight<FP8>(vw[i][2], vw[i][3]), w[1], o[i], 0, 0, 0);
         }
+        vb_now = vb_next;
+        if constexpr (more)
+            fetch_values(t + NW, vb_now);
+    };
+    if (t0 < t_end)
+    {
+        int t = t0;
+        for (; t + NW < t_end; t += NW)
+            step(t, std::true_type{});
+        step(t, std::false_type{});
     }
 
     // the waves' parts -> one
@@ -288,14 +382,17 @@ __global__ __launch_bounds__(256) void rows_kernel(const tllm_paged_attention_pa
         ls[wave][r] = l;
     }
     __syncthreads();
-    const float m_all = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), m_use = m_all == -INFINITY ? 0.f : m_all;
-    const float mine = __builtin_amdgcn_exp2f(m - m_use) * (v_ref * (1.f / kPScale));
-    if (wave >= 2)
+    float m_all = ms[0][r];
+#pragma unroll
+    for (int w = 1; w < NW; ++w)
+        m_all = fmaxf(m_all, ms[w][r]);
+    const float mine = __builtin_amdgcn_exp2f(m - (m_all == -INFINITY ? 0.f : m_all)) * (v_ref * __builtin_amdgcn_exp2f(-kPShift));
+    if (wave >= kPlaces)
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
-            *reinterpret_cast<f32x4*>(&acc[wave - 2][r][16 * i + 4 * g]) = o[i] * mine;
+            *reinterpret_cast<f32x4*>(&acc[wave - kPlaces][r][16 * i + 4 * g]) = o[i] * mine;
     __syncthreads();
-    if (wave < 2)
+    if (wave < kPlaces)
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
         {
@@ -303,24 +400,29 @@ __global__ __launch_bounds__(256) void rows_kernel(const tllm_paged_attention_pa
             *at = *at + o[i] * mine;
         }
     __syncthreads();
-    for (int u = tid; u < 16 * DIM / 8; u += 256)
+    for (int u = tid; u < 16 * DIM / 4; u += 64 * NW)
     {
-        const int ur = u / (DIM / 8), d = u % (DIM / 8) * 8, urow = tile * 16 + ur;
+        const int ur = u / (DIM / 4), d = u % (DIM / 4) * 4, urow = tile * 16 + ur;
         if (urow >= rows)
             continue;
-        const float um = fmaxf(fmaxf(ms[0][ur], ms[1][ur]), fmaxf(ms[2][ur], ms[3][ur])), uu = um == -INFINITY ? 0.f : um;
+        float um = ms[0][ur];
+#pragma unroll
+        for (int w = 1; w < NW; ++w)
+            um = fmaxf(um, ms[w][ur]);
+        const float uu = um == -INFINITY ? 0.f : um;
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < NW; ++w)
             sum += ls[w][ur] * __builtin_amdgcn_exp2f(ms[w][ur] - uu);
-        const f32x4 a = *reinterpret_cast<const f32x4*>(&acc[0][ur][d]) + *reinterpret_cast<const f32x4*>(&acc[1][ur][d]);
-        const f32x4 c = *reinterpret_cast<const f32x4*>(&acc[0][ur][d + 4]) + *reinterpret_cast<const f32x4*>(&acc[1][ur][d + 4]);
+        f32x4 a = *reinterpret_cast<const f32x4*>(&acc[0][ur][d]);
+#pragma unroll
+        for (int i = 1; i < kPlaces; ++i)
+            a += *reinterpret_cast<const f32x4*>(&acc[i][ur][d]);
         const int utoken = urow / group, uh = head * group + urow - utoken * group;
         if (split.parts > 1)
         {
             const int64_t at = ((int64_t) (req.row0 + utoken) * p.q_heads + uh) * split.parts + part;
             *reinterpret_cast<f32x4*>(split.o + at * DIM + d) = a;
-            *reinterpret_cast<f32x4*>(split.o + at * DIM + d + 4) = c;
             if (d == 0)
             {
                 split.ml[2 * at] = um;
@@ -329,75 +431,327 @@ __global__ __launch_bounds__(256) void rows_kernel(const tllm_paged_attention_pa
             continue;
         }
         const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); // a row that saw nothing is 0, a NaN stays one
-        uint16_t* const to = static_cast<uint16_t*>(p.out) + (req.row0 + utoken) * p.out_row + uh * p.out_head + d;
-        *reinterpret_cast<uint4*>(to) = make_uint4(pack_out<BF16>(a[0] * inv, a[1] * inv), pack_out<BF16>(a[2] * inv, a[3] * inv),
-            pack_out<BF16>(c[0] * inv, c[1] * inv), pack_out<BF16>(c[2] * inv, c[3] * inv));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (req.row0 + utoken) * p.out_row + uh * p.out_head + d)
+            = make_uint2(pack_out<BF16>(a[0] * inv, a[1] * inv), pack_out<BF16>(a[2] * inv, a[3] * inv));
     }
 }
 
-// parts of the keys -> rows: a wave per row and head
+// a workgroup per request, key head and part of the keys: rows of one tile
+template <int DIM, bool BF16, bool FP8, int NW>
+__global__ __launch_bounds__(64 * NW) void rows_kernel(const tllm_paged_attention_params_t p, const int shift, const Split split)
+{
+    __shared__ f32x4 lds[RowsLds<DIM>::bytes(NW) / 16];
+    int id = blockIdx.x;
+    const int part = id % split.parts;
+    id /= split.parts;
+    const int head = id % p.kv_heads, b = id / p.kv_heads;
+    const Request req = request_of(p, b, shift);
+    if (req.rows > 0)
+        rows_body<DIM, BF16, FP8, NW>(p, shift, split, req, head, b, 0, part, reinterpret_cast<float*>(lds));
+}
+
+template <int DIM>
+struct TileForm
+{
+    static constexpr int kRt = DIM == 256 ? 1 : 2, kRows = 64 * kRt; // row tiles of a wave, rows of a workgroup of four
+    static constexpr int kKeyFrags = 4 * DIM / 32, kFrags = 2 * kKeyFrags; // of 1 KB: keys [part][k-step], values [channels / 16][k-step]
+    static constexpr int kLds = 2 * kFrags * 1024;
+};
+
+// Tiles of kRows rows of a request and key head.  Requests of at most 16 rows in the same batch take rows_body.
+template <int DIM, bool BF16, bool FP8>
+__global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tllm_paged_attention_params_t p, const int shift, const int row_tiles)
+{
+    using F = TileForm<DIM>;
+    constexpr int kSteps = DIM / 32, kOut = DIM / 16, RT = F::kRt;
+    extern __shared__ u32x4 frags[]; // [2][kFrags][64]
+    // workgroups go round the XCDs: the row tiles of one request and head follow each other on one XCD, whose L2 holds their keys; those with
+    // the most keys first
+    const int xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, pair = at8 / row_tiles * 8 + xcd, tile = row_tiles - 1 - at8 % row_tiles;
+    if (pair >= p.n_seqs * p.kv_heads)
+        return;
+    const int head = pair % p.kv_heads, b = pair / p.kv_heads, group = p.q_heads / p.kv_heads;
+    const Request req = request_of(p, b, shift);
+    const int rows = min(req.rows, p.max_new) * group;
+    if (tile * F::kRows >= rows)
+        return;
+    if (rows <= 16)
+        return rows_body<DIM, BF16, FP8, 4>(p, shift, Split{nullptr, nullptr, 1}, req, head, b, 0, 0, reinterpret_cast<float*>(frags));
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int first = req.len - req.rows;
+    // tiles of keys that rows [a, a + n) see
+    auto tiles_lo = [&](int a) { return p.window > 0 ? max(0, first + a / group + 1 - p.window) / kTile : 0; };
+    auto tiles_hi = [&](int a, int n) { return (max(0, first + min(a + n - 1, rows - 1) / group + 1) + kTile - 1) / kTile; };
+    const int row0 = tile * F::kRows, t_begin = tiles_lo(row0), t_end = tiles_hi(row0, F::kRows);
+    const int my0 = row0 + wave * 16 * RT;
+    const bool idle = my0 >= rows;
+    const int my_begin = idle ? t_end : tiles_lo(my0), my_end = idle ? t_end : tiles_hi(my0, 16 * RT);
+
+    const int page = 1 << shift;
+    const int64_t head_bytes = (int64_t) page * DIM, side_bytes = head_bytes * p.kv_heads;
+    const uint8_t* const pool = static_cast<const uint8_t*>(p.pool) + head * head_bytes;
+    const int32_t* const table = p.block_table + (int64_t) b * p.table_stride;
+    auto held = [&](int block) { return (uint32_t) block < (uint32_t) p.num_blocks; };
+
+    // The wave brings part `wave` of the keys and channels 16 (wave + 4 i) of the values, 16 bytes a lane and load, as rows_body reads them.
+    int kb = -1, vb = -1;
+    u32x4 kw[DIM / 64], vw[DIM / 64];
+    float ks_next = 0.f, vs_next = 0.f;
+    int vb_there = -1; // blocks of what has been sent for
+    auto blocks_of = [&](int t) {
+        const int kk = t * kTile + 16 * (r >> 2), vk = t * kTile + 16 * g;
+        kb = kk < req.len ? table[kk >> shift] : -1;
+        vb = vk < req.len ? table[vk >> shift] : -1;
+    };
+    auto send = [&](int t) {
+        const uint8_t* const ka = pool + (int64_t) (held(kb) ? kb : 0) * 2 * side_bytes + (((t * kTile + 16 * (r >> 2)) & (page - 1)) + (r & 3) + 4 * wave) * DIM + 16 * g;
+        const uint8_t* const va = pool + ((int64_t) (held(vb) ? vb : 0) * 2 + 1) * side_bytes + (16 * wave + r) * page + ((t * kTile + 16 * g) & (page - 1));
+#pragma unroll
+        for (int j = 0; j < DIM / 64; ++j)
+        {
+            kw[j] = *reinterpret_cast<const u32x4*>(ka + 64 * j);
+            vw[j] = *reinterpret_cast<const u32x4*>(va + 64 * j * page);
+        }
+        const float* const s_at = p.scales + (int64_t) (held(vb) ? vb : 0) * 2 * p.kv_heads + head;
+        ks_next = s_at[0];
+        vs_next = s_at[p.kv_heads];
+        vb_there = vb;
+    };
+    auto land = [&](int t) {
+        u32x4* const to = frags + (t & 1) * F::kFrags * 64 + lane;
+        const int keep = held(vb_there) ? req.len - (t * kTile + 16 * g) : 0;
+        const bool whole = __builtin_amdgcn_ballot_w64(keep < 16) == 0;
+#pragma unroll
+        for (int j = 0; j < DIM / 64; ++j)
+        {
+            u32x4* const kt = to + (wave * kSteps + 2 * j) * 64;
+            kt[0] = __builtin_bit_cast(u32x4, eight<FP8>(kw[j][0], kw[j][1]));
+            kt[64] = __builtin_bit_cast(u32x4, eight<FP8>(kw[j][2], kw[j][3]));
+            u32x4 v = vw[j];
+            if (!whole)
+                v = cut(v, keep);
+            u32x4* const vt = to + (F::kKeyFrags + (wave + 4 * j) * 2) * 64;
+            vt[0] = __builtin_bit_cast(u32x4, eight<FP8>(v[0], v[1]));
+            vt[64] = __builtin_bit_cast(u32x4, eight<FP8>(v[2], v[3]));
+        }
+    };
+
+    f16x8 q[RT][kSteps];
+    f32x4 o[RT][kOut];
+    float factor[RT], m[RT], l[RT], v_ref = 0.f;
+    int seen[RT], from[RT];
+    if (t_begin < t_end)
+    {
+        blocks_of(t_begin);
+        send(t_begin);
+        if (t_begin + 1 < t_end)
+            blocks_of(t_begin + 1);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+    {
+        const int row = my0 + 16 * i + r, token = row / group, qh = head * group + row - token * group;
+        const bool live = row < rows;
+        const uint16_t* const q_row = live ? static_cast<const uint16_t*>(p.q) + (req.row0 + token) * p.q_row + qh * p.q_head : nullptr;
+        factor[i] = load_query<DIM, BF16>(q[i], q_row, g) * p.scale * kLog2e;
+        seen[i] = live ? first + token + 1 : 0x7fffffff;
+        from[i] = live && p.window > 0 ? seen[i] - p.window : 0;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < kOut; ++d)
+            o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float ks = 0.f, vs = 0.f;
+    bool v_in = false;
+    if (t_begin < t_end)
+    {
+        land(t_begin);
+        v_in = held(vb_there);
+        ks = v_in ? ks_next : 0.f;
+        vs = v_in ? vs_next : 0.f;
+    }
+    __syncthreads();
+    auto step = [&](int t, auto more) { // the last one by itself, as in rows_body
+        if constexpr (more)
+        {
+            send(t + 1);
+            if (t + 2 < t_end)
+                blocks_of(t + 2);
+        }
+        if (t >= my_begin && t < my_end)
+        {
+            const u32x4* const kt = frags + (t & 1) * F::kFrags * 64 + lane;
+            const u32x4* const vt = kt + F::kKeyFrags * 64;
+            const int vk = t * kTile + 16 * g;
+            float s[RT][16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                f32x4 c[RT];
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j)
+                {
+                    const f16x8 a = join(kt[(i * kSteps + j) * 64]);
+#pragma unroll
+                    for (int n = 0; n < RT; ++n)
+                        c[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[n][j], j ? c[n] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                }
+#pragma unroll
+                for (int n = 0; n < RT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[n][4 * i + e] = c[n][e];
+            }
+            const TileScales scales = scales_of(ks, vs, v_ref);
+            f16x8 w[RT][2];
+#pragma unroll
+            for (int n = 0; n < RT; ++n)
+                soften(s[n], w[n], m[n], l[n], o[n], scales, factor[n], __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen[n] || vk < from[n]) == 0, v_in, vk, from[n], seen[n]);
+#pragma unroll
+            for (int d = 0; d < kOut; ++d)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                {
+                    const f16x8 a = join(vt[(2 * d + h) * 64]);
+#pragma unroll
+                    for (int n = 0; n < RT; ++n)
+                        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[n][h], o[n][d], 0, 0, 0);
+                }
+        }
+        if constexpr (more)
+        {
+            land(t + 1); // its half was read in the round before
+            v_in = held(vb_there);
+            ks = v_in ? ks_next : 0.f;
+            vs = v_in ? vs_next : 0.f;
+            __syncthreads();
+        }
+    };
+    if (t_begin < t_end)
+    {
+        for (int t = t_begin; t + 1 < t_end; ++t)
+            step(t, std::true_type{});
+        step(t_end - 1, std::false_type{});
+    }
+#pragma unroll
+    for (int n = 0; n < RT; ++n)
+    {
+        const float sum = groups_sum(l[n]);
+        const int row = my0 + 16 * n + r, token = row / group, qh = head * group + row - token * group;
+        if (row >= rows)
+            continue;
+        const float inv = (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) * (v_ref * __builtin_amdgcn_exp2f(-kPShift));
+        uint16_t* const to = static_cast<uint16_t*>(p.out) + (req.row0 + token) * p.out_row + qh * p.out_head + 4 * g;
+#pragma unroll
+        for (int d = 0; d < kOut; ++d)
+            *reinterpret_cast<uint2*>(to + 16 * d) = make_uint2(pack_out<BF16>(o[n][d][0] * inv, o[n][d][1] * inv), pack_out<BF16>(o[n][d][2] * inv, o[n][d][3] * inv));
+    }
+}
+
+// Parts of the keys -> rows: a workgroup per row and head, its waves take the parts in turn.
 template <int DIM, bool BF16>
 __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_params_t p, const int shift, const Split split)
 {
     constexpr int kPer = DIM / 64;
-    const int lane = threadIdx.x & 63;
-    int64_t id = (int64_t) blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = (int) (id % p.q_heads);
+    __shared__ float os[4][DIM];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int id = blockIdx.x;
+    const int h = id % p.q_heads;
     id /= p.q_heads;
-    const int i = (int) (id % p.max_new), b = (int) (id / p.max_new);
-    if (b >= p.n_seqs)
-        return;
+    const int i = id % p.max_new, b = id / p.max_new;
     const Request req = request_of(p, b, shift);
     if (i >= req.rows)
         return;
     const int64_t at = ((int64_t) (req.row0 + i) * p.q_heads + h) * split.parts;
-    float m = -INFINITY;
-    for (int s = 0; s < split.parts; ++s)
-        m = fmaxf(m, split.ml[2 * (at + s)]);
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float sum = 0.f, o[kPer] = {};
-    for (int s = 0; s < split.parts; ++s)
+    float m = -INFINITY, l = 0.f; // of part `lane`: there are 64 at most
+    if (lane < split.parts)
     {
-        const float w = __builtin_amdgcn_exp2f(split.ml[2 * (at + s)] - m_use);
-        sum += w * split.ml[2 * (at + s) + 1];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-            o[e] += w * split.o[(at + s) * DIM + lane * kPer + e];
+        const float2 v = reinterpret_cast<const float2*>(split.ml)[at + lane];
+        m = v.x;
+        l = v.y;
     }
-    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-    uint16_t* const to = static_cast<uint16_t*>(p.out) + (req.row0 + i) * p.out_row + h * p.out_head + lane * kPer;
+    const float m_all = wave_max(m), w = __builtin_amdgcn_exp2f(m - (m_all == -INFINITY ? 0.f : m_all)), sum = wave_sum(w * l);
+    float o[kPer] = {};
+    for (int s0 = 0; s0 < split.parts; s0 += 16) // four loads of a wave at a time
+    {
+        float x[4][kPer];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            const int s = s0 + 4 * k + wave;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                x[k][e] = s < split.parts ? split.o[(at + s) * DIM + lane * kPer + e] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            const float ws = __shfl(w, min(s0 + 4 * k + wave, 63), 64);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                o[e] += ws * x[k][e];
+        }
+    }
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
-        to[e] = BF16 ? f2bf(o[e] * inv) : f2h(o[e] * inv);
+        os[wave][lane * kPer + e] = o[e];
+    __syncthreads();
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+    for (int d = threadIdx.x; d < DIM; d += 256)
+    {
+        const float v = (os[0][d] + os[1][d] + os[2][d] + os[3][d]) * inv;
+        static_cast<uint16_t*>(p.out)[(req.row0 + i) * p.out_row + h * p.out_head + d] = BF16 ? f2bf(v) : f2h(v);
+    }
 }
 
-// Workgroups that the keys are split into: as many as fill the chip twice over, a part no shorter than 512 keys.
+bool one_tile(const tllm_paged_attention_params_t& p) // no request has more than 16 rows of a key head
+{
+    return (int64_t) p.max_new * (p.q_heads / p.kv_heads) <= 16;
+}
+
+// Workgroups that the keys are split into, where a request's rows are one tile: enough for every CU to have several (their contexts differ in
+// length), a part no shorter than 256 keys.
 int parts_of(const tllm_paged_attention_params_t& p)
 {
-    const int row_tiles = ((int64_t) p.max_new * (p.q_heads / p.kv_heads) + 15) / 16;
-    if (row_tiles > 1)
+    if (!one_tile(p))
         return 1;
     const int64_t groups = (int64_t) p.n_seqs * p.kv_heads;
     const int64_t keys = p.window > 0 ? std::min(p.window, p.max_kv) : p.max_kv;
-    const int64_t want = 2 * launch_util::device_cus() / groups, most = keys / 512;
+    const int64_t want = (PARTS_WANT * launch_util::device_cus() + groups - 1) / groups, most = keys / PARTS_KEYS;
     return (int) std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64));
+}
+
+template <int DIM, bool BF16, bool FP8>
+void launch_form(const tllm_paged_attention_params_t& p, void* workspace, hipStream_t stream)
+{
+    const int shift = __builtin_ctz((unsigned) p.page_size);
+    const int64_t pairs = (int64_t) p.n_seqs * p.kv_heads;
+    if (!one_tile(p))
+    {
+        using F = TileForm<DIM>;
+        const int row_tiles = (int) (((int64_t) p.max_new * (p.q_heads / p.kv_heads) + F::kRows - 1) / F::kRows);
+        launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&tile_kernel<DIM, BF16, FP8>), F::kLds);
+        tile_kernel<DIM, BF16, FP8><<<(unsigned) ((pairs + 7) / 8 * 8 * row_tiles), 256, F::kLds, stream>>>(p, shift, row_tiles);
+        return;
+    }
+    const int parts = parts_of(p);
+    Split split = {static_cast<float*>(workspace), nullptr, parts};
+    if (parts > 1)
+        split.ml = split.o + (int64_t) p.n_rows * p.q_heads * parts * DIM;
+    rows_kernel<DIM, BF16, FP8, 4><<<(unsigned) (pairs * parts), 256, 0, stream>>>(p, shift, split);
+    if (parts > 1)
+        merge_kernel<DIM, BF16><<<(unsigned) ((int64_t) p.n_seqs * p.max_new * p.q_heads), 256, 0, stream>>>(p, shift, split);
 }
 
 template <int DIM, bool BF16>
 void launch_dim(const tllm_paged_attention_params_t& p, void* workspace, hipStream_t stream)
 {
-    const int shift = __builtin_ctz((unsigned) p.page_size), parts = parts_of(p);
-    const int row_tiles = (int) (((int64_t) p.max_new * (p.q_heads / p.kv_heads) + 15) / 16);
-    Split split = {static_cast<float*>(workspace), nullptr, parts};
-    if (parts > 1)
-        split.ml = split.o + (int64_t) p.n_rows * p.q_heads * parts * DIM;
-    const int64_t grid = (int64_t) p.n_seqs * p.kv_heads * row_tiles * parts;
     if (p.cache_type == TLLM_FP8)
-        rows_kernel<DIM, BF16, true><<<(unsigned) grid, 256, 0, stream>>>(p, shift, row_tiles, split);
+        launch_form<DIM, BF16, true>(p, workspace, stream);
     else
-        rows_kernel<DIM, BF16, false><<<(unsigned) grid, 256, 0, stream>>>(p, shift, row_tiles, split);
-    if (parts > 1)
-        merge_kernel<DIM, BF16><<<(unsigned) (((int64_t) p.n_seqs * p.max_new * p.q_heads + 3) / 4), 256, 0, stream>>>(p, shift, split);
+        launch_form<DIM, BF16, false>(p, workspace, stream);
 }
 } // namespace
 

@@ -108,10 +108,10 @@ bool attention_fits(const tllm_paged_attention_params_t* p)
     TLLM_REFUSE(p->table_stride < p->max_blocks, "%s: table_stride %lld is less than max_blocks %d", me, (long long) p->table_stride, p->max_blocks);
     TLLM_REFUSE(p->max_new < 1 || p->max_new > kMaxRows, "%s: max_new %d outside [1, %d]", me, p->max_new, kMaxRows);
     TLLM_REFUSE(p->max_kv < 0 || p->window < 0, "%s: a negative max_kv or window", me);
-    TLLM_REFUSE(!(p->scale > -1e30f && p->scale < 1e30f), "%s: the scale is not finite", me);
+    TLLM_REFUSE(!(p->scale >= 0.f && p->scale < 1e30f), "%s: the scale is negative or not finite", me);
     TLLM_REFUSE(!p->block_table || !p->cu_tokens || !p->kv_lens || !aligned(p->block_table, 4) || !aligned(p->cu_tokens, 4) || !aligned(p->kv_lens, 4),
         "%s: tables and lengths are null or not 4-byte aligned", me);
-    TLLM_REFUSE((int64_t) p->n_seqs * p->kv_heads * (((int64_t) p->max_new * (p->q_heads / p->kv_heads) + 15) / 16) > INT32_MAX / 64
+    TLLM_REFUSE((int64_t) p->n_seqs * p->kv_heads * (((int64_t) p->max_new * (p->q_heads / p->kv_heads) + 15) / 16) > INT32_MAX / 64 - 8
             || (int64_t) p->n_seqs * p->max_new * p->q_heads > INT32_MAX,
         "%s: %d requests of up to %d rows are more than one launch takes", me, p->n_seqs, p->max_new);
     return p->n_rows == 0 || (rows_fit(me, "q", p->q, p->q_row, p->q_head) && rows_fit(me, "out", p->out, p->out_row, p->out_head));
