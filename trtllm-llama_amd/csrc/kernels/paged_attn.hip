@@ -9,8 +9,9 @@
 //   P goes from the first product's registers into the second's as it is.  16 keys lie in one page, so a lane has one key scale and one value
 //   scale per tile.
 // 8-bit elements become fp16 exactly (int8: 0x6400 | (q + 128) = 1152 + q; e4m3: the convert instruction).  Scales enter in fp32: the key's with the
-// softmax scale behind the first product; the value's, relative to the largest value scale so far and times 2^15, in the exponent of the
-// weight (P <= 2^15: nothing overflows, and a weight keeps its 11 bits until its page's scale is 2^-29 of another's).
+// softmax scale behind the first product; the value's, relative to the largest value scale so far and times 2^7, in the exponent of the
+// weight.  m is brought along only when a score is more than 8 (a factor of 2^8) above it: a weight is at most 2^15, nothing overflows, it keeps
+// its 11 bits until its page's scale is 2^-21 of another's, and in most tiles no lane asks another for anything.
 //   rows_body   16 rows: four or eight waves take tiles in turn, straight from memory into registers, and join through LDS.  Single tokens are bound by
 //               the cache's bytes; the keys are also split over workgroups, whose parts merge_kernel joins.
 //   tile_kernel 64 or 128 rows: the waves share the tiles, which they bring to LDS as fp16 fragments, the next one while this one is computed.  Prompts
@@ -35,12 +36,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kPShift = 15.f; // see above
+constexpr float kPShift = 7.f, kSlack = 8.f; // see above
 constexpr int kTile = 64;
-#ifndef PARTS_WANT
-#define PARTS_WANT 8
-#define PARTS_KEYS 256
-#endif
 
 __device__ __forceinline__ f16x8 join(u32x4 w)
 {
@@ -174,24 +171,33 @@ struct Split
     int parts;
 };
 
-// What a tile's pages say to a lane: their scales, and how its weights are scaled for the second product.
+// The value scales: the reference that O is in units of, and what a tile's pages say to a lane.
+struct Reference
+{
+    float v = 0.f, log_v = 0.f;
+};
 struct TileScales
 {
     float ks, vs;
     float lift, drop; // weights are formed times 2^lift; 2^-lift
     float back;       // what O has to be multiplied by as the reference grows
 };
-__device__ __forceinline__ TileScales scales_of(float ks, float vs, float& v_ref)
+__device__ __forceinline__ TileScales scales_of(float ks, float vs, Reference& ref)
 {
     TileScales t;
     t.ks = ks;
     t.vs = vs;
-    const float v_new = fmaxf(v_ref, groups_max(vs));
-    t.back = v_new > v_ref ? v_ref / v_new : 1.f;
+    t.back = 1.f;
+    if (__builtin_amdgcn_ballot_w64(vs > ref.v))
+    {
+        const float v_new = fmaxf(ref.v, groups_max(vs));
+        t.back = ref.v / v_new;
+        ref.v = v_new;
+        ref.log_v = __builtin_amdgcn_logf(v_new);
+    }
     // below 2^-60 of the reference a page's weights are 0 in fp16 either way; l still has to see them
-    t.lift = v_new > 0.f ? fmaxf(__builtin_amdgcn_logf(vs / v_new) + kPShift, -60.f) : 0.f;
+    t.lift = fmaxf(__builtin_amdgcn_logf(vs) - ref.log_v + kPShift, -60.f);
     t.drop = __builtin_amdgcn_exp2f(-t.lift);
-    v_ref = v_new;
     return t;
 }
 
@@ -213,17 +219,18 @@ __device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], float& m, 
 #pragma unroll
     for (int i = 1; i < 16; ++i)
         top = fmaxf(top, s[i]);
-    const float m_new = fmaxf(m, groups_max(top * f)), m_use = m_new == -INFINITY ? 0.f : m_new; // f >= 0
-    if (__builtin_amdgcn_ballot_w64(m_new != m || t.back != 1.f))
+    top *= f; // f >= 0
+    if (__builtin_amdgcn_ballot_w64(top > m + kSlack || t.back != 1.f))
     {
-        const float alpha = __builtin_amdgcn_exp2f(m - m_use), back = alpha * t.back;
+        const float m_new = fmaxf(m, groups_max(top));
+        const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new), back = alpha * t.back;
         l *= alpha;
+        m = m_new;
 #pragma unroll
         for (int i = 0; i < N; ++i)
             o[i] *= back;
     }
-    m = m_new;
-    const float shift = t.lift - m_use;
+    const float shift = t.lift - (m == -INFINITY ? 0.f : m);
     float sum = 0.f;
     u32x4 p[2];
 #pragma unroll
@@ -268,8 +275,8 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
     const int t_begin = t_lo + min(n_tiles, part * per), t_end = t_lo + min(n_tiles, (part + 1) * per);
 
     const int page = 1 << shift;
-    const int64_t head_bytes = (int64_t) page * DIM, side_bytes = head_bytes * p.kv_heads;
-    const uint8_t* const pool = static_cast<const uint8_t*>(p.pool) + head * head_bytes;
+    const uint32_t head_bytes = page * DIM, side_bytes = head_bytes * p.kv_heads; // at most 32 MB
+    const uint8_t* const pool = static_cast<const uint8_t*>(p.pool) + (int64_t) head * head_bytes;
     const int32_t* const table = p.block_table + (int64_t) b * p.table_stride;
 
     // What a tile needs of memory, each part sent for as soon as its registers are free: blocks two tiles ahead, keys and scales behind the
@@ -284,18 +291,18 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
     };
     auto held = [&](int block) { return (uint32_t) block < (uint32_t) p.num_blocks; };
     auto fetch_keys = [&](int t) {
-        const uint8_t* const at = pool + (int64_t) (held(kb) ? kb : 0) * 2 * side_bytes + (((t * kTile + 16 * (r >> 2)) & (page - 1)) + (r & 3)) * DIM + 16 * g;
+        const uint8_t* const at = pool + (uint64_t) (uint32_t) (held(kb) ? kb : 0) * (2 * side_bytes) + (((t * kTile + 16 * (r >> 2)) & (page - 1)) + (r & 3)) * DIM + 16 * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < DIM / 64; ++j)
                 kw[i][j] = *reinterpret_cast<const u32x4*>(at + 4 * i * DIM + 64 * j);
-        const float* const s_at = p.scales + (int64_t) (held(vb) ? vb : 0) * 2 * p.kv_heads + head;
+        const float* const s_at = p.scales + (uint64_t) (uint32_t) (held(vb) ? vb : 0) * (uint32_t) (2 * p.kv_heads) + head;
         ks_next = s_at[0];
         vs_next = s_at[p.kv_heads];
     };
     auto fetch_values = [&](int t, int block) {
-        const uint8_t* const at = pool + ((int64_t) (held(block) ? block : 0) * 2 + 1) * side_bytes + r * page + ((t * kTile + 16 * g) & (page - 1));
+        const uint8_t* const at = pool + (uint64_t) (uint32_t) (held(block) ? block : 0) * (2 * side_bytes) + side_bytes + r * page + ((t * kTile + 16 * g) & (page - 1));
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
             vw[i] = *reinterpret_cast<const u32x4*>(at + 16 * i * page);
@@ -319,7 +326,8 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
 #pragma unroll
     for (int i = 0; i < kOut; ++i)
         o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f, v_ref = 0.f;
+    float m = -INFINITY, l = 0.f;
+    Reference ref;
     // The last tile of a wave sends for nothing.  It is a body of its own: with the loads under a condition inside one loop the compiler's scheduler
     // has written over registers of the values that were still to be read (hipcc 7.2, seen in the assembly and by the tests).
     auto step = [&](int t, auto more) {
@@ -348,7 +356,7 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
             if (t + 2 * NW < t_end)
                 blocks_of(t + 2 * NW);
         }
-        const TileScales scales = scales_of(ks, vs, v_ref);
+        const TileScales scales = scales_of(ks, vs, ref);
         const int keep = v_in ? req.len - vk : 0;
         f16x8 w[2];
         soften(s, w, m, l, o, scales, factor, __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen || vk < from) == 0, v_in, vk, from, seen);
@@ -386,7 +394,7 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
 #pragma unroll
     for (int w = 1; w < NW; ++w)
         m_all = fmaxf(m_all, ms[w][r]);
-    const float mine = __builtin_amdgcn_exp2f(m - (m_all == -INFINITY ? 0.f : m_all)) * (v_ref * __builtin_amdgcn_exp2f(-kPShift));
+    const float mine = __builtin_amdgcn_exp2f(m - (m_all == -INFINITY ? 0.f : m_all)) * (ref.v * __builtin_amdgcn_exp2f(-kPShift));
     if (wave >= kPlaces)
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
@@ -489,8 +497,8 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
     const int my_begin = idle ? t_end : tiles_lo(my0), my_end = idle ? t_end : tiles_hi(my0, 16 * RT);
 
     const int page = 1 << shift;
-    const int64_t head_bytes = (int64_t) page * DIM, side_bytes = head_bytes * p.kv_heads;
-    const uint8_t* const pool = static_cast<const uint8_t*>(p.pool) + head * head_bytes;
+    const uint32_t head_bytes = page * DIM, side_bytes = head_bytes * p.kv_heads; // at most 32 MB
+    const uint8_t* const pool = static_cast<const uint8_t*>(p.pool) + (int64_t) head * head_bytes;
     const int32_t* const table = p.block_table + (int64_t) b * p.table_stride;
     auto held = [&](int block) { return (uint32_t) block < (uint32_t) p.num_blocks; };
 
@@ -505,15 +513,15 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
         vb = vk < req.len ? table[vk >> shift] : -1;
     };
     auto send = [&](int t) {
-        const uint8_t* const ka = pool + (int64_t) (held(kb) ? kb : 0) * 2 * side_bytes + (((t * kTile + 16 * (r >> 2)) & (page - 1)) + (r & 3) + 4 * wave) * DIM + 16 * g;
-        const uint8_t* const va = pool + ((int64_t) (held(vb) ? vb : 0) * 2 + 1) * side_bytes + (16 * wave + r) * page + ((t * kTile + 16 * g) & (page - 1));
+        const uint8_t* const ka = pool + (uint64_t) (uint32_t) (held(kb) ? kb : 0) * (2 * side_bytes) + (((t * kTile + 16 * (r >> 2)) & (page - 1)) + (r & 3) + 4 * wave) * DIM + 16 * g;
+        const uint8_t* const va = pool + (uint64_t) (uint32_t) (held(vb) ? vb : 0) * (2 * side_bytes) + side_bytes + (16 * wave + r) * page + ((t * kTile + 16 * g) & (page - 1));
 #pragma unroll
         for (int j = 0; j < DIM / 64; ++j)
         {
             kw[j] = *reinterpret_cast<const u32x4*>(ka + 64 * j);
             vw[j] = *reinterpret_cast<const u32x4*>(va + 64 * j * page);
         }
-        const float* const s_at = p.scales + (int64_t) (held(vb) ? vb : 0) * 2 * p.kv_heads + head;
+        const float* const s_at = p.scales + (uint64_t) (uint32_t) (held(vb) ? vb : 0) * (uint32_t) (2 * p.kv_heads) + head;
         ks_next = s_at[0];
         vs_next = s_at[p.kv_heads];
         vb_there = vb;
@@ -539,7 +547,8 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
 
     f16x8 q[RT][kSteps];
     f32x4 o[RT][kOut];
-    float factor[RT], m[RT], l[RT], v_ref = 0.f;
+    float factor[RT], m[RT], l[RT];
+    Reference ref;
     int seen[RT], from[RT];
     if (t_begin < t_end)
     {
@@ -604,7 +613,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
                     for (int e = 0; e < 4; ++e)
                         s[n][4 * i + e] = c[n][e];
             }
-            const TileScales scales = scales_of(ks, vs, v_ref);
+            const TileScales scales = scales_of(ks, vs, ref);
             f16x8 w[RT][2];
 #pragma unroll
             for (int n = 0; n < RT; ++n)
@@ -642,7 +651,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
         const int row = my0 + 16 * n + r, token = row / group, qh = head * group + row - token * group;
         if (row >= rows)
             continue;
-        const float inv = (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) * (v_ref * __builtin_amdgcn_exp2f(-kPShift));
+        const float inv = (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) * (ref.v * __builtin_amdgcn_exp2f(-kPShift));
         uint16_t* const to = static_cast<uint16_t*>(p.out) + (req.row0 + token) * p.out_row + qh * p.out_head + 4 * g;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
@@ -711,16 +720,17 @@ bool one_tile(const tllm_paged_attention_params_t& p) // no request has more tha
     return (int64_t) p.max_new * (p.q_heads / p.kv_heads) <= 16;
 }
 
-// Workgroups that the keys are split into, where a request's rows are one tile: enough for every CU to have several (their contexts differ in
-// length), a part no shorter than 256 keys.
+// Workgroups that the keys are split into, where a request's rows are one tile.  Fewer requests and key heads than CUs: two a CU.  More of them: the
+// split only evens out contexts of different lengths, and joining costs more than that unless they are long (48 x 8 heads over 4000 to 8000
+// keys of 128: 117 us in 3 parts, 125 in 6; 64 x 8 over 300 to 600: 21 us whole, 28 in two; one of 32 heads over 1032: 10.7 us in 8 parts, 12.4 in 4).
 int parts_of(const tllm_paged_attention_params_t& p)
 {
     if (!one_tile(p))
         return 1;
-    const int64_t groups = (int64_t) p.n_seqs * p.kv_heads;
+    const int64_t groups = (int64_t) p.n_seqs * p.kv_heads, cus = launch_util::device_cus();
     const int64_t keys = p.window > 0 ? std::min(p.window, p.max_kv) : p.max_kv;
-    const int64_t want = (PARTS_WANT * launch_util::device_cus() + groups - 1) / groups, most = keys / PARTS_KEYS;
-    return (int) std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64));
+    const int64_t want = ((groups < cus ? 2 : 4) * cus + groups - 1) / groups, least = groups >= cus ? 2048 : groups * 4 >= cus ? 512 : 128;
+    return (int) std::max<int64_t>(1, std::min<int64_t>(std::min(want, keys / least), 64));
 }
 
 template <int DIM, bool BF16, bool FP8>
