@@ -473,9 +473,11 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
     using F = TileForm<DIM>;
     constexpr int kSteps = DIM / 32, kOut = DIM / 16, RT = F::kRt;
     extern __shared__ u32x4 frags[]; // [2][kFrags][64]
-    // workgroups go round the XCDs: the row tiles of one request and head follow each other on one XCD, whose L2 holds their keys; those with
-    // the most keys first
-    const int xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, pair = at8 / row_tiles * 8 + xcd, tile = row_tiles - 1 - at8 % row_tiles;
+    // Workgroups go round the XCDs: the row tiles of one request and head follow each other on one XCD, whose L2 holds their keys.  Those with the
+    // most keys first, and the other way round in every second 32: workgroups 32 apart of an XCD meet on one CU (2048 tokens behind 1500, 32
+    // heads of 128: 125 us, 148 without)
+    const int xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, pair = at8 / row_tiles * 8 + xcd;
+    const int tile = at8 >> 5 & 1 ? at8 % row_tiles : row_tiles - 1 - at8 % row_tiles;
     if (pair >= p.n_seqs * p.kv_heads)
         return;
     const int head = pair % p.kv_heads, b = pair / p.kv_heads, group = p.q_heads / p.kv_heads;
@@ -594,40 +596,59 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
             const u32x4* const kt = frags + (t & 1) * F::kFrags * 64 + lane;
             const u32x4* const vt = kt + F::kKeyFrags * 64;
             const int vk = t * kTile + 16 * g;
+            f32x4 c[RT][4];
+            // fragments are read a group of four ahead of their products: LDS answers behind some hundred cycles
             float s[RT][16];
+            u32x4 a[2][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < 4; ++j)
+                a[0][j] = kt[j * 64];
+#pragma unroll
+            for (int i = 0; i < F::kKeyFrags / 4; ++i) // four k-steps, of part i / (kSteps / 4)
             {
-                f32x4 c[RT];
+                if (i + 1 < F::kKeyFrags / 4)
 #pragma unroll
-                for (int j = 0; j < kSteps; ++j)
+                    for (int j = 0; j < 4; ++j)
+                        a[(i + 1) & 1][j] = kt[((i + 1) * 4 + j) * 64];
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
                 {
-                    const f16x8 a = join(kt[(i * kSteps + j) * 64]);
+                    const int part = (4 * i + j) / kSteps, step = (4 * i + j) % kSteps;
 #pragma unroll
                     for (int n = 0; n < RT; ++n)
-                        c[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[n][j], j ? c[n] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                        c[n][part] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(a[i & 1][j]), q[n][step], step ? c[n][part] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
                 }
-#pragma unroll
-                for (int n = 0; n < RT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[n][4 * i + e] = c[n][e];
+                __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int n = 0; n < RT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[n][i] = c[n][i / 4][i % 4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                a[0][j] = vt[j * 64];
             const TileScales scales = scales_of(ks, vs, ref);
             f16x8 w[RT][2];
 #pragma unroll
             for (int n = 0; n < RT; ++n)
                 soften(s[n], w[n], m[n], l[n], o[n], scales, factor[n], __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen[n] || vk < from[n]) == 0, v_in, vk, from[n], seen[n]);
 #pragma unroll
-            for (int d = 0; d < kOut; ++d)
+            for (int i = 0; i < kOut / 2; ++i) // channels 32 i .. + 31
+            {
+                if (i + 1 < kOut / 2)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                {
-                    const f16x8 a = join(vt[(2 * d + h) * 64]);
+                    for (int j = 0; j < 4; ++j)
+                        a[(i + 1) & 1][j] = vt[((i + 1) * 4 + j) * 64];
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int n = 0; n < RT; ++n)
-                        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[n][h], o[n][d], 0, 0, 0);
-                }
+                        o[n][2 * i + j / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(a[i & 1][j]), w[n][j & 1], o[n][2 * i + j / 2], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         if constexpr (more)
         {
