@@ -256,25 +256,49 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(const tllm_group_matmul_pa
     const uint32_t lds0 = (uint32_t) (uintptr_t) (lds_t*) lds;
 
     // chunk c of a k-tile: x (row tile c / 4, k-step c % 4), then weights, then scales; a wave brings chunks wave, wave + 8, .. (the last one once
-    // more where they do not divide)
+    // more where they do not divide).  Each has an address that moves by the same step every k-tile.
+    const char* from[F::kPerWave];
+    uint32_t moves[F::kPerWave];
+    int k_of[F::kPerWave]; // of x: the lane's first k of the first tile, -1 for the others
+#pragma unroll
+    for (int i = 0; i < F::kPerWave; ++i)
+    {
+        const int c = min(i * 8 + wave, F::kChunks - 1);
+        k_of[i] = -1;
+        if (c < F::kX)
+        {
+            k_of[i] = 32 * (c & 3) + 8 * g;
+            from[i] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(p.x) + (int64_t) min((tile_m * 8 + (c >> 2)) * 16 + r, p.rows - 1) * p.ldx + k_of[i]);
+            moves[i] = 256;
+        }
+        else if (c < F::kX + F::kW)
+        {
+            from[i] = reinterpret_cast<const char*>(static_cast<const uint4*>(p.packed) + (int64_t) min(n0 + c - F::kX, n_tiles - 1) * k_tiles * 64 + lane);
+            moves[i] = 1024;
+        }
+        else
+        {
+            from[i] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(p.scales) + (int64_t) (c - F::kX - F::kW) * n_all + min(n0 * 16 + lane * 8, n_all - 8));
+            moves[i] = F::kGroups * n_all * 2;
+        }
+    }
     auto bring = [&](int t) {
         const uint32_t to = lds0 + (t % kStages) * F::kStageBytes;
+        const bool tail = t == k_tiles - 1; // k may end inside: x is 0 there, as the weights are; a scale that is none is the last one's
 #pragma unroll
         for (int i = 0; i < F::kPerWave; ++i)
         {
             const int c = min(i * 8 + wave, F::kChunks - 1);
-            const void* from;
-            if (c < F::kX)
+            const void* at = from[i];
+            if (tail)
             {
-                const int k = t * 128 + 32 * (c & 3) + 8 * g;
-                from = static_cast<const uint16_t*>(p.x) + (int64_t) min((tile_m * 8 + (c >> 2)) * 16 + r, p.rows - 1) * p.ldx + k;
-                from = k < p.k ? from : static_cast<const void*>(kZeros);
+                if (c < F::kX)
+                    at = t * 128 + k_of[i] < p.k ? at : kZeros;
+                else if (c >= F::kX + F::kW)
+                    at = from[i] - (int64_t) max(t * F::kGroups + c - F::kX - F::kW - (groups - 1), 0) * n_all * 2;
             }
-            else if (c < F::kX + F::kW)
-                from = static_cast<const uint4*>(p.packed) + ((int64_t) min(n0 + c - F::kX, n_tiles - 1) * k_tiles + t) * 64 + lane;
-            else
-                from = static_cast<const uint16_t*>(p.scales) + (int64_t) min(t * F::kGroups + c - F::kX - F::kW, groups - 1) * n_all + min(n0 * 16 + lane * 8, n_all - 8);
-            dma16(from, to + c * 1024);
+            dma16(at, to + c * 1024);
+            from[i] += moves[i];
         }
     };
     f32x4 y[NT][4];
@@ -320,24 +344,37 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(const tllm_group_matmul_pa
                         sum[i] = product<BF16>(ones, b[j][i], sum[i]);
                 }
             }
+            // the products of output tile n are under way while n + 1 is converted and n - 1 is scaled
+            u32x4 w[2][kSteps];
+            f32x4 acc[2][4];
+            uint2 scale[2];
+            auto convert = [&](int n) {
+                const uint32_t* const words = reinterpret_cast<const uint32_t*>(ws + n * 64) + q * kSteps;
+                scale[n & 1] = *reinterpret_cast<const uint2*>(ss + q * 1024 + n * 32);
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j)
+                    w[n & 1][j] = weights8<BF16>(words[j]);
+            };
+            auto add = [&](int n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    scaled_add<BF16>(y[n][i], acc[n & 1][i], sum[i], scale[n & 1]);
+            };
+            convert(0);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
             {
-                const uint32_t* const words = reinterpret_cast<const uint32_t*>(ws + n * 64) + q * kSteps;
-                const uint2 s = *reinterpret_cast<const uint2*>(ss + q * 1024 + n * 32);
-                f32x4 acc[4];
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j)
-                {
-                    const u32x4 a = weights8<BF16>(words[j]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        acc[i] = product<BF16>(a, b[j][i], j ? acc[i] : zero);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    scaled_add<BF16>(y[n][i], acc[i], sum[i], s);
+                        acc[n & 1][i] = product<BF16>(w[n & 1][j], b[j][i], j ? acc[n & 1][i] : zero);
+                if (n > 0)
+                    add(n - 1);
+                if (n + 1 < NT)
+                    convert(n + 1);
             }
+            add(NT - 1);
         }
     }
     const bool whole = p.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;

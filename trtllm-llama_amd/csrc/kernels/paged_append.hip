@@ -126,32 +126,35 @@ __device__ __forceinline__ void load_unit(float (&x)[16], const uint16_t* row, c
 
 // Chunk of rows -> LDS: the row before it, the chunk, and as many behind it as a run can go on for.  What is no place of the pool, or
 // has no angle, becomes -1.
-__device__ __forceinline__ void load_slots(const tllm_paged_append_params_t& p, int* slots, int t0, int count, int shift)
+__device__ __forceinline__ void load_slots(const tllm_paged_append_params_t& p, int* slots, int* places, int t0, int count, int shift)
 {
     const uint32_t end = (uint32_t) p.num_blocks << shift;
     for (int i = threadIdx.x; i < count; i += blockDim.x)
     {
         const int t = t0 - 1 + i;
-        int s = -1;
+        int s = -1, at = 0;
         if (t >= 0 && t < p.n_rows)
         {
             s = p.slot_map[t];
-            if ((uint32_t) s >= end || (p.rot_dim && (uint32_t) p.positions[t] >= (uint32_t) p.rope_len))
+            if (p.rot_dim)
+                at = p.positions[t];
+            if ((uint32_t) s >= end || (p.rot_dim && (uint32_t) at >= (uint32_t) p.rope_len))
                 s = -1;
         }
         slots[i] = s;
+        places[i] = at;
     }
 }
 
 template <int DIM, bool BF16, bool FP8>
 __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_paged_append_params_t p, const int shift, const int chunk)
 {
-    __shared__ int slots[kMaxChunk + kMaxPage + 1];
+    __shared__ int slots[kMaxChunk + kMaxPage + 1], places[kMaxChunk + kMaxPage + 1];
     __shared__ float red[32];
     const int page = 1 << shift, t0 = blockIdx.x * chunk, tid = threadIdx.x;
     const int kv_jobs = 2 * p.kv_heads;
     const bool pairs = p.rope_pairs != 0;
-    load_slots(p, slots, t0, chunk + page + 1, shift);
+    load_slots(p, slots, places, t0, chunk + page + 1, shift);
     __syncthreads();
 
     if ((int) blockIdx.y >= kv_jobs) // queries: a unit a thread
@@ -164,7 +167,7 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
         const int hu = u - r * per_row, h = hu / kUnits;
         const Unit at = unit_at(hu - h * kUnits, p.rot_dim, pairs);
         float x[16];
-        load_unit<BF16>(x, static_cast<const uint16_t*>(p.q) + t * p.q_row + h * p.q_head, at, p.rope, p.rot_dim, p.positions[t], pairs);
+        load_unit<BF16>(x, static_cast<const uint16_t*>(p.q) + t * p.q_row + h * p.q_head, at, p.rope, p.rot_dim, places[1 + r], pairs);
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -199,8 +202,18 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
         float* const scale_at = p.scales + (block * 2 + which) * p.kv_heads + head;
         const float old = off ? *scale_at : 0.f;
 
+        // everything that is read of memory is sent for here, before the first of it is waited for
         float x[32];
         float big = kFloor;
+        uint4 was[2] = {}; // the thread's two pieces of a page of values, where they are not wholly new
+        const int v_first = tid / (DIM / 2) * 16, lo = off - v_first, hi = off + n - v_first; // of its 16 places those in [lo, hi) are new, those before held
+        uint4* const v_at = reinterpret_cast<uint4*>(base + tid % (DIM / 2) * 2 * page + v_first);
+        const bool partly = which == 1 && tid < threads && hi > 0 && (lo > 0 || hi < 16);
+        if (partly)
+        {
+            was[0] = *v_at;
+            was[1] = v_at[page / 16];
+        }
         if (which == 0)
         {
             constexpr int kUnits = DIM / 16;
@@ -213,7 +226,7 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
                 float y[16] = {};
                 if (tid < threads && row < n)
                     load_unit<BF16>(y, static_cast<const uint16_t*>(p.k) + (t + row) * p.k_row + head * p.k_head, at, p.rope, p.rot_dim,
-                        p.rot_dim ? p.positions[t + row] : 0, pairs);
+                        places[1 + r + row], pairs);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     x[half * 16 + i] = finite<BF16>(y[i]);
@@ -271,20 +284,11 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
         }
         else if (tid < threads)
         {
-            constexpr int kPairs = DIM / 2;
-            const int d = tid % kPairs * 2, first = tid / kPairs * 16;
-            const int lo = off - first, hi = off + n - first; // of the thread's 16 places those in [lo, hi) are new, those before held
             if (hi > 0 && (lo < 16 || grew))
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
                 {
-                    uint4* const to = reinterpret_cast<uint4*>(base + (d + c) * page + first);
-                    uint32_t w[4] = {0, 0, 0, 0};
-                    if (lo > 0 || hi < 16)
-                    {
-                        const uint4 was = *to;
-                        w[0] = was.x, w[1] = was.y, w[2] = was.z, w[3] = was.w;
-                    }
+                    uint32_t w[4] = {was[c].x, was[c].y, was[c].z, was[c].w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                     {
@@ -301,7 +305,7 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
                         }
                         w[i] = out;
                     }
-                    *to = make_uint4(w[0], w[1], w[2], w[3]);
+                    v_at[c * (page / 16)] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
         }
         r += n - 1;
