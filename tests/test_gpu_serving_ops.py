@@ -337,6 +337,13 @@ def test_attention_split_over_workgroups(spans, max_kv, kind, dtype, size):
     check_attention(np.random.default_rng(size), kind, dtype, 64, size, 1, 3, spans, max_kv=max_kv, spare_rows=1)
 
 
+@pytest.mark.parametrize('size', [64, 256])
+def test_attention_of_many_workgroups(size):
+    """More than 32 row tiles an XCD, in numbers that do not divide it: every row is computed, and once."""
+    spans = [(290, 270), (400, 300), (130, 130)] if size == 64 else [(140, 140), (200, 180)]
+    check_attention(np.random.default_rng(size), 'int8', 'fp16', 64, size, 32 if size == 64 else 64, 1, spans)
+
+
 def test_attention_rows_that_see_nothing():
     """More rows than cached tokens: the first ones stand before the cache's beginning.  Lengths below zero and beyond the table."""
     rng = np.random.default_rng(8)

@@ -474,10 +474,10 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
     constexpr int kSteps = DIM / 32, kOut = DIM / 16, RT = F::kRt;
     extern __shared__ u32x4 frags[]; // [2][kFrags][64]
     // Workgroups go round the XCDs: the row tiles of one request and head follow each other on one XCD, whose L2 holds their keys.  Those with the
-    // most keys first, and the other way round in every second 32: workgroups 32 apart of an XCD meet on one CU (2048 tokens behind 1500, 32
-    // heads of 128: 125 us, 148 without)
-    const int xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, pair = at8 / row_tiles * 8 + xcd;
-    const int tile = at8 >> 5 & 1 ? at8 % row_tiles : row_tiles - 1 - at8 % row_tiles;
+    // most keys first, and the other way round where a pair of request and head begins in an odd 32: workgroups 32 apart of an XCD meet on
+    // one CU (2048 tokens behind 1500, 32 heads of 128: 125 us, 148 without)
+    const int xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, order = at8 % row_tiles, pair = at8 / row_tiles * 8 + xcd;
+    const int tile = (at8 - order) >> 5 & 1 ? order : row_tiles - 1 - order;
     if (pair >= p.n_seqs * p.kv_heads)
         return;
     const int head = pair % p.kv_heads, b = pair / p.kv_heads, group = p.q_heads / p.kv_heads;

@@ -40,7 +40,7 @@ def _lib():
 
 def on_device(index: int, call, *args):
     """call(*args, stream) with device `index` as the current one and torch's current stream of it."""
-    current = torch.cuda.current_device()
+    current = torch._C._cuda_getDevice()
     if current == index:
         return call(*args, torch._C._cuda_getCurrentRawStream(index))
     torch.cuda.set_device(index)
@@ -205,7 +205,7 @@ class PagedKV8Cache(object):
                 raise ValueError('queries are only rotated here, and there is no rope table')
             q_at, q_heads, q_row, q_head = _rows('q', q, rows, None, size, dtype, index)
             if q_out is None:
-                q_out = torch.empty((rows, q_heads, size), dtype=dtype, device=q.device)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             o_at, _, o_row, o_head = _rows('q_out', q_out, rows, q_heads, size, dtype, index, True)
         p = _APPEND.pack(rows, heads, q_heads, size, self.page_size, self.blocks, act, self._type, rot, 1 if rope_pairs else 0, angle_rows, k_at, v_at, q_at, o_at,
                          k_row, k_head, v_row, v_head, q_row, q_head, o_row, o_head, _ints('slot_map', slot_map, rows, index), places, angles, *self._at)
@@ -226,7 +226,7 @@ class PagedKV8Cache(object):
         q_at, heads, q_row, q_head = _rows('q', q, rows, None, size, dtype, index)
         table, stride, wide = _table(block_table, n, index)
         if out is None:
-            out = torch.empty((rows, heads, size), dtype=dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         o_at, _, o_row, o_head = _rows('out', out, rows, heads, size, dtype, index, True)
         p = _ATTENTION.pack(n, rows, heads, self.kv_heads, size, self.page_size, self.blocks, wide, act, self._type, max_new,
                             wide * self.page_size if max_kv is None else max_kv, window, size**-0.5 if scale is None else scale, stride, q_row, q_head, o_row, o_head,
