@@ -344,6 +344,13 @@ def test_attention_of_many_workgroups(size):
     check_attention(np.random.default_rng(size), 'int8', 'fp16', 64, size, 32 if size == 64 else 64, 1, spans)
 
 
+@pytest.mark.parametrize('kind,dtype,size', [('int8', 'fp16', 128), ('fp8', 'bf16', 64), ('int8', 'bf16', 256)])
+@pytest.mark.parametrize('window', [0, 1500])
+def test_attention_prompts_split_over_workgroups(window, kind, dtype, size):
+    """Few row tiles over long contexts, beside a single token, an empty request and one that sees little."""
+    check_attention(np.random.default_rng(size), kind, dtype, 64, size, 1, 2, [(5000, 40), (3100, 1), (0, 0), (70, 30), (9, 20)], window=window, max_kv=9000, spare_rows=1)
+
+
 def test_attention_rows_that_see_nothing():
     """More rows than cached tokens: the first ones stand before the cache's beginning.  Lengths below zero and beyond the table."""
     rng = np.random.default_rng(8)

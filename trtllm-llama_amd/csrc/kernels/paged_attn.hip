@@ -463,21 +463,23 @@ struct TileForm
 {
     static constexpr int kRt = DIM == 256 ? 1 : 2, kRows = 64 * kRt; // row tiles of a wave, rows of a workgroup of four
     static constexpr int kKeyFrags = 4 * DIM / 32, kFrags = 2 * kKeyFrags; // of 1 KB: keys [part][k-step], values [channels / 16][k-step]
-    static constexpr int kLds = 2 * kFrags * 1024;
+    static constexpr int kAhead = DIM == 256 ? 2 : 4; // fragments that are read ahead of their products
+    // Tiles that LDS holds: two, one computed and one arriving; of heads of 256 one, so that two workgroups fit a CU
+    static constexpr int kBuffers = DIM == 256 ? 1 : 2, kLds = kBuffers * kFrags * 1024;
 };
 
 // Tiles of kRows rows of a request and key head.  Requests of at most 16 rows in the same batch take rows_body.
 template <int DIM, bool BF16, bool FP8>
-__global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tllm_paged_attention_params_t p, const int shift, const int row_tiles)
+__global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm_paged_attention_params_t p, const int shift, const int row_tiles, const Split split)
 {
     using F = TileForm<DIM>;
     constexpr int kSteps = DIM / 32, kOut = DIM / 16, RT = F::kRt;
-    extern __shared__ u32x4 frags[]; // [2][kFrags][64]
+    extern __shared__ u32x4 frags[]; // [kBuffers][kFrags][64]
     // Workgroups go round the XCDs: the row tiles of one request and head follow each other on one XCD, whose L2 holds their keys.  Those with the
     // most keys first, and the other way round where a pair of request and head begins in an odd 32: workgroups 32 apart of an XCD meet on
     // one CU (2048 tokens behind 1500, 32 heads of 128: 125 us, 148 without)
     const int xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, order = at8 % row_tiles, pair = at8 / row_tiles * 8 + xcd;
-    const int tile = (at8 - order) >> 5 & 1 ? order : row_tiles - 1 - order;
+    const int tile = (at8 - order) >> 5 & 1 ? order : row_tiles - 1 - order, part = blockIdx.y;
     if (pair >= p.n_seqs * p.kv_heads)
         return;
     const int head = pair % p.kv_heads, b = pair / p.kv_heads, group = p.q_heads / p.kv_heads;
@@ -486,14 +488,15 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
     if (tile * F::kRows >= rows)
         return;
     if (rows <= 16)
-        return rows_body<DIM, BF16, FP8, 4>(p, shift, Split{nullptr, nullptr, 1}, req, head, b, 0, 0, reinterpret_cast<float*>(frags));
+        return rows_body<DIM, BF16, FP8, 4>(p, shift, split, req, head, b, 0, part, reinterpret_cast<float*>(frags));
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int first = req.len - req.rows;
     // tiles of keys that rows [a, a + n) see
     auto tiles_lo = [&](int a) { return p.window > 0 ? max(0, first + a / group + 1 - p.window) / kTile : 0; };
     auto tiles_hi = [&](int a, int n) { return (max(0, first + min(a + n - 1, rows - 1) / group + 1) + kTile - 1) / kTile; };
-    const int row0 = tile * F::kRows, t_begin = tiles_lo(row0), t_end = tiles_hi(row0, F::kRows);
+    const int row0 = tile * F::kRows, t_lo = tiles_lo(row0), n_tiles = max(0, tiles_hi(row0, F::kRows) - t_lo), per = (n_tiles + split.parts - 1) / split.parts;
+    const int t_begin = t_lo + min(n_tiles, part * per), t_end = t_lo + min(n_tiles, (part + 1) * per);
     const int my0 = row0 + wave * 16 * RT;
     const bool idle = my0 >= rows;
     const int my_begin = idle ? t_end : tiles_lo(my0), my_end = idle ? t_end : tiles_hi(my0, 16 * RT);
@@ -529,7 +532,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
         vb_there = vb;
     };
     auto land = [&](int t) {
-        u32x4* const to = frags + (t & 1) * F::kFrags * 64 + lane;
+        u32x4* const to = frags + (t & (F::kBuffers - 1)) * F::kFrags * 64 + lane;
         const int keep = held(vb_there) ? req.len - (t * kTile + 16 * g) : 0;
         const bool whole = __builtin_amdgcn_ballot_w64(keep < 16) == 0;
 #pragma unroll
@@ -593,28 +596,29 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
         }
         if (t >= my_begin && t < my_end)
         {
-            const u32x4* const kt = frags + (t & 1) * F::kFrags * 64 + lane;
+            const u32x4* const kt = frags + (t & (F::kBuffers - 1)) * F::kFrags * 64 + lane;
             const u32x4* const vt = kt + F::kKeyFrags * 64;
             const int vk = t * kTile + 16 * g;
             f32x4 c[RT][4];
-            // fragments are read a group of four ahead of their products: LDS answers behind some hundred cycles
+            // fragments are read kAhead before their products: LDS answers behind some hundred cycles
+            constexpr int kAhead = F::kAhead;
             float s[RT][16];
-            u32x4 a[2][4];
+            u32x4 a[2][kAhead];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < kAhead; ++j)
                 a[0][j] = kt[j * 64];
 #pragma unroll
-            for (int i = 0; i < F::kKeyFrags / 4; ++i) // four k-steps, of part i / (kSteps / 4)
+            for (int i = 0; i < F::kKeyFrags / kAhead; ++i)
             {
-                if (i + 1 < F::kKeyFrags / 4)
+                if (i + 1 < F::kKeyFrags / kAhead)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        a[(i + 1) & 1][j] = kt[((i + 1) * 4 + j) * 64];
+                    for (int j = 0; j < kAhead; ++j)
+                        a[(i + 1) & 1][j] = kt[((i + 1) * kAhead + j) * 64];
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < kAhead; ++j)
                 {
-                    const int part = (4 * i + j) / kSteps, step = (4 * i + j) % kSteps;
+                    const int part = (kAhead * i + j) / kSteps, step = (kAhead * i + j) % kSteps;
 #pragma unroll
                     for (int n = 0; n < RT; ++n)
                         c[n][part] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(a[i & 1][j]), q[n][step], step ? c[n][part] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
@@ -627,7 +631,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
                 for (int i = 0; i < 16; ++i)
                     s[n][i] = c[n][i / 4][i % 4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < kAhead; ++j)
                 a[0][j] = vt[j * 64];
             const TileScales scales = scales_of(ks, vs, ref);
             f16x8 w[RT][2];
@@ -635,24 +639,29 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
             for (int n = 0; n < RT; ++n)
                 soften(s[n], w[n], m[n], l[n], o[n], scales, factor[n], __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen[n] || vk < from[n]) == 0, v_in, vk, from[n], seen[n]);
 #pragma unroll
-            for (int i = 0; i < kOut / 2; ++i) // channels 32 i .. + 31
+            for (int i = 0; i < F::kKeyFrags / kAhead; ++i) // as many fragments of values: channels 16 (f / 2), keys 32 (f % 2)
             {
-                if (i + 1 < kOut / 2)
+                if (i + 1 < F::kKeyFrags / kAhead)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        a[(i + 1) & 1][j] = vt[((i + 1) * 4 + j) * 64];
+                    for (int j = 0; j < kAhead; ++j)
+                        a[(i + 1) & 1][j] = vt[((i + 1) * kAhead + j) * 64];
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < kAhead; ++j)
 #pragma unroll
                     for (int n = 0; n < RT; ++n)
-                        o[n][2 * i + j / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(a[i & 1][j]), w[n][j & 1], o[n][2 * i + j / 2], 0, 0, 0);
+                    {
+                        f32x4& to = o[n][(kAhead * i + j) / 2];
+                        to = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(a[i & 1][j]), w[n][j & 1], to, 0, 0, 0);
+                    }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         if constexpr (more)
         {
-            land(t + 1); // its half was read in the round before
+            if constexpr (F::kBuffers == 1)
+                __syncthreads(); // every wave has read the tile
+            land(t + 1); // two buffers: its one was read in the round before
             v_in = held(vb_there);
             ks = v_in ? ks_next : 0.f;
             vs = v_in ? vs_next : 0.f;
@@ -672,7 +681,21 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void tile_kernel(const tll
         const int row = my0 + 16 * n + r, token = row / group, qh = head * group + row - token * group;
         if (row >= rows)
             continue;
-        const float inv = (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) * (ref.v * __builtin_amdgcn_exp2f(-kPShift));
+        const float unit = ref.v * __builtin_amdgcn_exp2f(-kPShift);
+        if (split.parts > 1)
+        {
+            const int64_t at = ((int64_t) (req.row0 + token) * p.q_heads + qh) * split.parts + part;
+#pragma unroll
+            for (int d = 0; d < kOut; ++d)
+                *reinterpret_cast<f32x4*>(split.o + at * DIM + 16 * d + 4 * g) = o[n][d] * unit;
+            if (g == 0)
+            {
+                split.ml[2 * at] = m[n];
+                split.ml[2 * at + 1] = sum;
+            }
+            continue;
+        }
+        const float inv = (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) * unit;
         uint16_t* const to = static_cast<uint16_t*>(p.out) + (req.row0 + token) * p.out_row + qh * p.out_head + 4 * g;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
@@ -741,16 +764,32 @@ bool one_tile(const tllm_paged_attention_params_t& p) // no request has more tha
     return (int64_t) p.max_new * (p.q_heads / p.kv_heads) <= 16;
 }
 
-// Workgroups that the keys are split into, where a request's rows are one tile.  Fewer requests and key heads than CUs: two a CU.  More of them: the
-// split only evens out contexts of different lengths, and joining costs more than that unless they are long (48 x 8 heads over 4000 to 8000
-// keys of 128: 117 us in 3 parts, 125 in 6; 64 x 8 over 300 to 600: 21 us whole, 28 in two; one of 32 heads over 1032: 10.7 us in 8 parts, 12.4 in 4).
+int row_tiles_of(const tllm_paged_attention_params_t& p) // of tile_kernel
+{
+    const int rows = p.head_size == 256 ? TileForm<256>::kRows : TileForm<128>::kRows;
+    return (int) (((int64_t) p.max_new * (p.q_heads / p.kv_heads) + rows - 1) / rows);
+}
+
+// Workgroups that the keys are split into.
+// Requests of one tile of rows: with fewer requests and key heads than CUs two a CU.  With more of them the split only evens out contexts of
+// different lengths, and joining costs more than that unless they are long (64 x 8 heads over 300 to 600 keys of 128: 21 us whole, 28 in
+// two parts; 48 x 8 over 4000 to 8000: 115 in three, 126 whole; one of 32 heads over 1032: 10.7 in 8 parts, 12.4 in 4).
+// More rows: what fills two places on every CU, where their tiles do not (443 tokens of one head over 57000 keys: 7 tiles).
 int parts_of(const tllm_paged_attention_params_t& p)
 {
-    if (!one_tile(p))
-        return 1;
-    const int64_t groups = (int64_t) p.n_seqs * p.kv_heads, cus = launch_util::device_cus();
-    const int64_t keys = p.window > 0 ? std::min(p.window, p.max_kv) : p.max_kv;
-    const int64_t want = ((groups < cus ? 2 : 4) * cus + groups - 1) / groups, least = groups >= cus ? 2048 : groups * 4 >= cus ? 512 : 128;
+    const int64_t pairs = (int64_t) p.n_seqs * p.kv_heads, cus = launch_util::device_cus();
+    const int64_t keys = p.window > 0 ? std::min<int64_t>((int64_t) p.window + p.max_new, p.max_kv) : p.max_kv;
+    int64_t want, least;
+    if (one_tile(p))
+    {
+        want = ((pairs < cus ? 2 : 4) * cus + pairs - 1) / pairs;
+        least = pairs >= cus ? 2048 : pairs * 4 >= cus ? 512 : 128;
+    }
+    else
+    {
+        want = 2 * cus / (pairs * row_tiles_of(p));
+        least = 1024;
+    }
     return (int) std::max<int64_t>(1, std::min<int64_t>(std::min(want, keys / least), 64));
 }
 
@@ -759,19 +798,19 @@ void launch_form(const tllm_paged_attention_params_t& p, void* workspace, hipStr
 {
     const int shift = __builtin_ctz((unsigned) p.page_size);
     const int64_t pairs = (int64_t) p.n_seqs * p.kv_heads;
-    if (!one_tile(p))
-    {
-        using F = TileForm<DIM>;
-        const int row_tiles = (int) (((int64_t) p.max_new * (p.q_heads / p.kv_heads) + F::kRows - 1) / F::kRows);
-        launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&tile_kernel<DIM, BF16, FP8>), F::kLds);
-        tile_kernel<DIM, BF16, FP8><<<(unsigned) ((pairs + 7) / 8 * 8 * row_tiles), 256, F::kLds, stream>>>(p, shift, row_tiles);
-        return;
-    }
     const int parts = parts_of(p);
     Split split = {static_cast<float*>(workspace), nullptr, parts};
     if (parts > 1)
         split.ml = split.o + (int64_t) p.n_rows * p.q_heads * parts * DIM;
-    rows_kernel<DIM, BF16, FP8, 4><<<(unsigned) (pairs * parts), 256, 0, stream>>>(p, shift, split);
+    if (one_tile(p))
+        rows_kernel<DIM, BF16, FP8, 4><<<(unsigned) (pairs * parts), 256, 0, stream>>>(p, shift, split);
+    else
+    {
+        using F = TileForm<DIM>;
+        const int row_tiles = row_tiles_of(p);
+        launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&tile_kernel<DIM, BF16, FP8>), F::kLds);
+        tile_kernel<DIM, BF16, FP8><<<dim3((unsigned) ((pairs + 7) / 8 * 8 * row_tiles), parts), 256, F::kLds, stream>>>(p, shift, row_tiles, split);
+    }
     if (parts > 1)
         merge_kernel<DIM, BF16><<<(unsigned) ((int64_t) p.n_seqs * p.max_new * p.q_heads), 256, 0, stream>>>(p, shift, split);
 }
