@@ -184,6 +184,39 @@ def test_append_to_the_bit(page, size, heads, spans, dtype, kind):
     c.same()
 
 
+@pytest.mark.parametrize('spans', [[(5, 1100)], [(i, 1) for i in range(300)] + [(0, 900)], [(100, 3000), (0, 1), (31, 1), (63, 2), (0, 1300)]], ids=['one', 'tokens', 'prompts'])
+def test_append_of_many_rows(spans):
+    """Workgroups that look for runs in 16 rows, and in a page of rows."""
+    rng = np.random.default_rng(len(spans))
+    page, size, heads, blocks = 32, 64, 8, sum(-(-(a + n) // 32) for a, n in spans)
+    c = Cache(rng, blocks, page, heads, size, 'int8')
+    slots, _ = slots_of(rng, spans, page, blocks)
+    k, kf = values(rng, (len(slots), heads, size), 'fp16')
+    v, vf = values(rng, (len(slots), heads, size), 'fp16')
+    c.gpu.append(k.cuda(), v.cuda(), gpu(slots))
+    O.append(c.pool, c.scales, kf, vf, slots, page, 'int8', 65504)
+    c.same()
+
+
+def test_append_and_attention_beyond_32_bits():
+    """A pool of more than 2^32 bytes: pages at its end hold and give back what pages at the beginning of a small one do."""
+    rng = np.random.default_rng(6)
+    page, size, heads, n = 128, 128, 8, 17500  # 4.6 GB
+    far = P.PagedKV8Cache(torch.empty((n, 2, heads, page * size), dtype=torch.int8, device='cuda'), torch.zeros((n, 2, heads), device='cuda'), page, size)
+    near = P.PagedKV8Cache.empty(4, page, heads, size)
+    assert far.pool.numel() > 2**32
+    x = torch.from_numpy(rng.standard_normal((300, 3 * heads, size)).astype(np.float32)).half().cuda()
+    at = np.arange(300)
+    outs = []
+    for cache, ids in ((near, [2, 0, 3]), (far, [n - 1, n - 3, n - 2])):
+        slots = gpu([ids[t // page] * page + t % page for t in at])
+        cache.append(x[:, heads:2 * heads], x[:, 2 * heads:], slots)
+        table = gpu([ids])
+        outs.append([cache.attention(x[:, :heads], table, gpu([0, 300]), gpu([300]), 300), cache.attention(x[:1, :heads], table, gpu([0, 1]), gpu([290]), 1),
+                     cache.pool[ids[0]], cache.pool[ids[1]], cache.scales[ids[:2]]])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 @pytest.mark.parametrize('dtype,kind,pairs', [('fp16', 'int8', False), ('bf16', 'fp8', True), ('fp16', 'fp8', False), ('bf16', 'int8', True)])
 @pytest.mark.parametrize('size,rot,q_heads', [(64, 64, 8), (128, 128, 4), (128, 32, 5), (256, 240, 2), (256, 16, 3)])
 def test_append_rotates(size, rot, q_heads, dtype, kind, pairs):

@@ -124,26 +124,28 @@ __device__ __forceinline__ void load_unit(float (&x)[16], const uint16_t* row, c
     }
 }
 
-// Chunk of rows -> LDS: the row before it, the chunk, and as many behind it as a run can go on for.  What is no place of the pool, or
-// has no angle, becomes -1.
-__device__ __forceinline__ void load_slots(const tllm_paged_append_params_t& p, int* slots, int* places, int t0, int count, int shift)
+// The slot of row t and its place in the rope table; what is no place of the pool, or has no angle, has slot -1.
+struct Row
 {
-    const uint32_t end = (uint32_t) p.num_blocks << shift;
-    for (int i = threadIdx.x; i < count; i += blockDim.x)
+    int slot, place;
+};
+__device__ __forceinline__ Row row_at(const tllm_paged_append_params_t& p, int t, int shift)
+{
+    Row r = {-1, 0};
+    if (t >= 0 && t < p.n_rows)
     {
-        const int t = t0 - 1 + i;
-        int s = -1, at = 0;
-        if (t >= 0 && t < p.n_rows)
-        {
-            s = p.slot_map[t];
-            if (p.rot_dim)
-                at = p.positions[t];
-            if ((uint32_t) s >= end || (p.rot_dim && (uint32_t) at >= (uint32_t) p.rope_len))
-                s = -1;
-        }
-        slots[i] = s;
-        places[i] = at;
+        r.slot = p.slot_map[t];
+        if (p.rot_dim)
+            r.place = p.positions[t];
+        if ((uint32_t) r.slot >= (uint32_t) p.num_blocks << shift || (p.rot_dim && (uint32_t) r.place >= (uint32_t) p.rope_len))
+            r.slot = -1;
     }
+    return r;
+}
+
+__device__ __forceinline__ bool begins(int slot, int before, int page) // a run
+{
+    return slot >= 0 && !(before >= 0 && before + 1 == slot && (slot & (page - 1)) != 0);
 }
 
 template <int DIM, bool BF16, bool FP8>
@@ -154,7 +156,25 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
     const int page = 1 << shift, t0 = blockIdx.x * chunk, tid = threadIdx.x;
     const int kv_jobs = 2 * p.kv_heads;
     const bool pairs = p.rope_pairs != 0;
-    load_slots(p, slots, places, t0, chunk + page + 1, shift);
+    if ((int) blockIdx.y < kv_jobs)
+    {
+        // most chunks of a prompt have no run's beginning: every wave sees that by itself
+        bool any = false;
+        for (int i = 0; i < chunk && !any; i += 63)
+        {
+            const int here = i + (tid & 63) - 1, slot = here < chunk ? row_at(p, t0 + here, shift).slot : -1;
+            const int before = __shfl_up(slot, 1, 64);
+            any = __builtin_amdgcn_ballot_w64((tid & 63) > 0 && begins(slot, before, page)) != 0;
+        }
+        if (!any)
+            return;
+    }
+    for (int i = tid; i < chunk + page + 1; i += blockDim.x) // the row before the chunk, the chunk, and as many behind it as a run can go on for
+    {
+        const Row at = row_at(p, t0 - 1 + i, shift);
+        slots[i] = at.slot;
+        places[i] = at.place;
+    }
     __syncthreads();
 
     if ((int) blockIdx.y >= kv_jobs) // queries: a unit a thread
@@ -185,7 +205,7 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
     {
         const int s0 = __builtin_amdgcn_readfirstlane(slots[1 + r]), before = __builtin_amdgcn_readfirstlane(slots[r]);
         const int off = s0 & (page - 1);
-        if (s0 < 0 || (before >= 0 && before + 1 == s0 && off != 0))
+        if (!begins(s0, before, page))
             continue; // nothing, or the middle of a run
         int n = 0; // rows of the run
         for (int j0 = 0; j0 < page - off; j0 += 64)
@@ -284,7 +304,21 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
         }
         else if (tid < threads)
         {
-            if (hi > 0 && (lo < 16 || grew))
+            if (n == 1 && !grew) // a token by itself: a byte a channel
+            {
+                if (lo >= 0 && lo < 16)
+                {
+                    float one[2] = {};
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (i == lo)
+                            one[0] = x[i], one[1] = x[16 + i];
+                    const uint32_t w = four<FP8>(one[0] / scale, one[1] / scale, 0.f, 0.f);
+                    reinterpret_cast<uint8_t*>(v_at)[lo] = (uint8_t) w;
+                    reinterpret_cast<uint8_t*>(v_at)[page + lo] = (uint8_t) (w >> 8);
+                }
+            }
+            else if (hi > 0 && (lo < 16 || grew))
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
                 {
@@ -316,9 +350,16 @@ template <int DIM, bool BF16>
 void launch_dim(const tllm_paged_append_params_t& p, hipStream_t stream)
 {
     const int shift = __builtin_ctz((unsigned) p.page_size), threads = std::max(64, p.page_size * DIM / 32);
-    // rows a workgroup looks for runs in: one, so that decoded tokens - a run each - are side by side, until there are so many workgroups that
-    // those without a run would be most of the time
-    const int chunk = (int64_t) p.n_rows * p.kv_heads <= 8192 ? 1 : p.page_size;
+    // Rows a workgroup looks for runs in.  The host does not know whether they are tokens (a run each, that want workgroups of their own) or
+    // prompts (a run a page, where workgroups without one are most of the time): one row while that makes few workgroups, up to 16 where the
+    // chip is full of them either way, a page where that leaves thousands (us at 1 / 8 / 16 / 64 rows, 8 heads of 128: 64 tokens 8 / 25 / 44 / 168,
+    // 512 tokens 42 / 34 / 52 / 178, a prompt of 1024 74 / 26 / 18 / 12, prompts of 5459 82 / 32 / 34 / 32)
+    const int64_t work = (int64_t) p.n_rows * p.kv_heads;
+    int chunk = 1;
+    while (chunk * 2 <= std::min(16, p.page_size) && chunk * 2 * 512 <= work)
+        chunk *= 2;
+    if (work >= 32768)
+        chunk = p.page_size;
     const int q_groups = p.q_heads ? (chunk * p.q_heads * (DIM / 16) + threads - 1) / threads : 0;
     const dim3 grid((p.n_rows + chunk - 1) / chunk, 2 * p.kv_heads + q_groups);
     if (p.cache_type == TLLM_FP8)
