@@ -99,7 +99,7 @@ __device__ __forceinline__ void dma16(const void* from, uint32_t lds_byte)
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(m0_keep) : "v"(from), "s"(lds_byte) : "memory");
 }
 
-// Up to 4 R rows: a workgroup has 16 NT outputs, its waves share the k-tiles out and join through LDS.  What it has to read is the weights, once;
+// 4 R rows x 16 NT outputs a workgroup; its waves share the k-tiles out and join through LDS.  What it has to read is the weights, once;
 // each CU also reads all of x, which is as much as its weights at 8 rows and 16 outputs and is why x comes by whole 256-byte pieces of the
 // rows that there are.  A wave has a ring of DEEP k-tiles in LDS, its own: no barrier, only the count of what is under way.
 template <int R, int NT>
@@ -120,7 +120,7 @@ __global__ __launch_bounds__((64 * FewForm<R, NT>::kWaves)) void few_rows_kernel
     extern __shared__ uint4 lds[];
     typedef __attribute__((address_space(3))) void lds_t;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int k_tiles = (p.k + 127) / 128, n_tiles = (p.n + 15) / 16, n_all = n_tiles * 16, n0 = blockIdx.x * NT;
+    const int k_tiles = (p.k + 127) / 128, n_tiles = (p.n + 15) / 16, n_all = n_tiles * 16, n0 = blockIdx.x * NT, m0 = blockIdx.y * 4 * R;
     const int groups = (p.k + GROUP - 1) / GROUP;
     const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -133,7 +133,7 @@ __global__ __launch_bounds__((64 * FewForm<R, NT>::kWaves)) void few_rows_kernel
         {
             // rows of 256 bytes, piece c of 16 bytes at c ^ row: the 16 rows of a fragment read 16 different places
             const int row = 4 * i + g, k = t * 128 + ((r ^ (row & 15)) << 3);
-            const void* from = static_cast<const uint16_t*>(p.x) + (int64_t) min(row, p.rows - 1) * p.ldx + k;
+            const void* from = static_cast<const uint16_t*>(p.x) + (int64_t) min(m0 + row, p.rows - 1) * p.ldx + k;
             dma16(k < p.k ? from : static_cast<const void*>(kZeros), to + i * 1024);
         }
 #pragma unroll
@@ -218,8 +218,8 @@ __global__ __launch_bounds__((64 * FewForm<R, NT>::kWaves)) void few_rows_kernel
 #pragma unroll
         for (int w = 1; w < F::kWaves; ++w)
             v += part[(w * NT * MT + u) * 64 + lane];
-        const int n = (n0 + u / MT) * 16 + 4 * g, m = u % MT * 16 + r;
-        if (m < p.rows)
+        const int n = (n0 + u / MT) * 16 + 4 * g, m = m0 + u % MT * 16 + r;
+        if (m < min(p.rows, m0 + 4 * R)) // fewer than 16 rows: the other lanes computed some of them again
             store4<BF16>(p, v, m, n);
     }
 }
@@ -400,23 +400,12 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(const tllm_group_matmul_pa
 }
 
 template <bool BF16, int GROUP, int NT>
-void launch_tiles(const tllm_group_matmul_params_t& p, int m_tiles, int n_parts, hipStream_t stream)
+void launch_tiles(const tllm_group_matmul_params_t& p, hipStream_t stream)
 {
     const size_t lds = kStages * TileForm<GROUP, NT>::kStageBytes;
+    const int m_tiles = (p.rows + 127) / 128, n_parts = (p.n + 64 * NT - 1) / (64 * NT);
     launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&tile_kernel<BF16, GROUP, NT>), lds);
     tile_kernel<BF16, GROUP, NT><<<m_tiles * n_parts, 512, lds, stream>>>(p, m_tiles, m_tiles * n_parts);
-}
-
-// 256 or 192 outputs a workgroup, one workgroup a CU: whichever gets by with less work in its rounds
-template <bool BF16, int GROUP>
-void launch_many(const tllm_group_matmul_params_t& p, hipStream_t stream)
-{
-    const int cus = launch_util::device_cus(), m_tiles = (p.rows + 127) / 128, n4 = (p.n + 255) / 256, n3 = (p.n + 191) / 192;
-    const int64_t rounds4 = ((int64_t) m_tiles * n4 + cus - 1) / cus, rounds3 = ((int64_t) m_tiles * n3 + cus - 1) / cus;
-    if (rounds3 * 3 < rounds4 * 4)
-        launch_tiles<BF16, GROUP, 3>(p, m_tiles, n3, stream);
-    else
-        launch_tiles<BF16, GROUP, 4>(p, m_tiles, n4, stream);
 }
 
 template <bool BF16, int GROUP, int R, int NT>
@@ -424,39 +413,64 @@ void launch_few(const tllm_group_matmul_params_t& p, hipStream_t stream)
 {
     using F = FewForm<R, NT>;
     launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&few_rows_kernel<BF16, GROUP, R, NT>), F::kLds);
-    few_rows_kernel<BF16, GROUP, R, NT><<<((p.n + 15) / 16 + NT - 1) / NT, 64 * F::kWaves, F::kLds, stream>>>(p);
+    const dim3 grid(((p.n + 15) / 16 + NT - 1) / NT, (p.rows + 4 * R - 1) / (4 * R));
+    few_rows_kernel<BF16, GROUP, R, NT><<<grid, 64 * F::kWaves, F::kLds, stream>>>(p);
 }
 
-// as few outputs a workgroup as give one workgroup a CU (a CU reads x once then), at most 64
-template <bool BF16, int GROUP, int R>
-void launch_rows(const tllm_group_matmul_params_t& p, hipStream_t stream)
+// The forms and what a k-tile of a workgroup takes in each (us, all CUs busy; measured over 24 to 1024 rows and 190 to 12288 outputs of fp16 with groups
+// of 128).  Every form has the CU's LDS to itself, so a product takes as many rounds as its workgroups take places, and the form with the
+// least time is the one to take: 1 x 4096 x 4096 in 256 workgroups of 16 outputs, 1024 x 11008 x 4096 in 464 tiles of 128 x 192 (121 us; 150 in tiles of
+// 256, 197 in the largest of the others), 67 x 190 x 10144 in 60 workgroups of 16 x 16 (8.5 us; 143 in tiles), 200 x 4096 x 4096 in 256 of 64 x 64
+// (20 us; 60 in tiles).
+struct Form
 {
-    const int cus = launch_util::device_cus(), n_tiles = (p.n + 15) / 16;
-    if (n_tiles <= cus)
-        launch_few<BF16, GROUP, R, 1>(p, stream);
-    else if (n_tiles <= 2 * cus)
-        launch_few<BF16, GROUP, R, 2>(p, stream);
-    else if (n_tiles <= 3 * cus)
-        launch_few<BF16, GROUP, R, 3>(p, stream);
-    else
-        launch_few<BF16, GROUP, R, 4>(p, stream);
+    int rows, outputs;
+    float us;
+};
+constexpr Form kForms[] = {{4, 16, .07f}, {4, 32, .10f}, {4, 48, .13f}, {4, 64, .17f}, {8, 16, .07f}, {8, 32, .10f}, {8, 48, .14f}, {8, 64, .18f}, {16, 16, .09f}, {16, 32, .13f},
+    {16, 48, .17f}, {16, 64, .21f}, {32, 16, .16f}, {32, 32, .24f}, {32, 48, .29f}, {32, 64, .33f}, {64, 16, .25f}, {64, 32, .34f}, {64, 48, .50f}, {64, 64, .58f}, {128, 192, 1.88f},
+    {128, 256, 2.33f}};
+
+int form_of(int rows, int n, int k)
+{
+    const int cus = launch_util::device_cus(), k_tiles = (k + 127) / 128;
+    int best = 0;
+    double least = 1e30;
+    for (int i = 0; i < (int) (sizeof(kForms) / sizeof(kForms[0])); ++i)
+    {
+        const Form& f = kForms[i];
+        const int64_t groups = (int64_t) ((n + f.outputs - 1) / f.outputs) * ((rows + f.rows - 1) / f.rows);
+        const double us = (double) ((groups + cus - 1) / cus) * (2. + k_tiles * (double) f.us); // 2: a round's first loads and its end
+        if (us < least)
+        {
+            least = us;
+            best = i;
+        }
+    }
+    return best;
 }
 
 template <bool BF16, int GROUP>
 void launch_form(const tllm_group_matmul_params_t& p, hipStream_t stream)
 {
-    if (p.rows <= 4)
-        launch_rows<BF16, GROUP, 1>(p, stream);
-    else if (p.rows <= 8)
-        launch_rows<BF16, GROUP, 2>(p, stream);
-    else if (p.rows <= 16)
-        launch_rows<BF16, GROUP, 4>(p, stream);
-    else if (p.rows <= 32)
-        launch_rows<BF16, GROUP, 8>(p, stream);
-    else if (p.rows <= 64)
-        launch_rows<BF16, GROUP, 16>(p, stream);
-    else
-        launch_many<BF16, GROUP>(p, stream);
+    const Form f = kForms[form_of(p.rows, p.n, p.k)];
+#define TLLM_FEW(R)                                                                                                    \
+    case 4 * R:                                                                                                        \
+        f.outputs == 16 ? launch_few<BF16, GROUP, R, 1>(p, stream)                                                     \
+            : f.outputs == 32 ? launch_few<BF16, GROUP, R, 2>(p, stream)                                               \
+            : f.outputs == 48 ? launch_few<BF16, GROUP, R, 3>(p, stream)                                               \
+                              : launch_few<BF16, GROUP, R, 4>(p, stream);                                              \
+        break;
+    switch (f.rows)
+    {
+        TLLM_FEW(1)
+        TLLM_FEW(2)
+        TLLM_FEW(4)
+        TLLM_FEW(8)
+        TLLM_FEW(16)
+    default: f.outputs == 192 ? launch_tiles<BF16, GROUP, 3>(p, stream) : launch_tiles<BF16, GROUP, 4>(p, stream);
+    }
+#undef TLLM_FEW
 }
 } // namespace
 
