@@ -469,6 +469,13 @@ def test_group_matmul(rows, n, k, group, dtype):
     check_product(np.random.default_rng(rows + n + k), rows, n, k, group, dtype)
 
 
+@pytest.mark.parametrize('group,dtype', [(128, 'fp16'), (32, 'bf16'), (64, 'fp16')])
+@pytest.mark.parametrize('rows,n', [(1, 1), (1, 4116), (1, 8195), (1, 12295), (1027, 1), (5, 4111), (5, 8207), (5, 12291), (1064, 17), (9, 4099), (17, 4118), (17, 6155), (1362, 65), (1381, 129), (17, 8196), (33, 6146), (1671, 130), (1633, 258), (33, 8197), (65, 6149), (129, 10943), (385, 12378)])
+def test_group_matmul_in_every_form(rows, n, group, dtype):
+    """Sizes at which each of the kernels' shapes is the quickest, k ending inside a tile."""
+    check_product(np.random.default_rng(n), rows, n, 288, group, dtype)
+
+
 @pytest.mark.parametrize('rows', [1, 9, 40, 300])
 @pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
 def test_group_matmul_strided(rows, dtype):
