@@ -387,8 +387,8 @@ def test_attention_prompts_split_over_workgroups(window, kind, dtype, size):
 def test_attention_rows_that_see_nothing():
     """More rows than cached tokens: the first ones stand before the cache's beginning.  Lengths below zero and beyond the table."""
     rng = np.random.default_rng(8)
-    for spans in ([(3, 5), (0, 4), (70, 90)], [(0, 1), (1, 2)], [(2, 40), (-5, 3)]):
-        got = check_attention(rng, 'int8', 'fp16', 16, 64, 1, 2, spans)
+    for spans, window in (([(3, 5), (0, 4), (70, 90)], 0), ([(0, 1), (1, 2)], 0), ([(2, 40), (-5, 3)], 0), ([(3, 50), (1, 3)], 2**31 - 1), ([(3, 50), (1, 3)], 2)):
+        got = check_attention(rng, 'int8', 'fp16', 16, 64, 1, 2, spans, window=window)
         assert (got[:max(spans[0][1] - spans[0][0], 0)] == 0).all()
 
 

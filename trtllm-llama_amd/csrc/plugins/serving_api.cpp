@@ -158,13 +158,22 @@ int32_t tllm_paged_append(const tllm_paged_append_params_t* p, tllm_stream_t str
     return guarded([&] { return !append_fits(p) || (p->n_rows && launch_paged_append(*p, reinterpret_cast<hipStream_t>(stream))); });
 }
 
+// what the kernels get: a window that no row can fill is none (and does not take positions out of range)
+static tllm_paged_attention_params_t as_launched(const tllm_paged_attention_params_t& p)
+{
+    tllm_paged_attention_params_t q = p;
+    if (q.window >= (int64_t) q.max_blocks * q.page_size)
+        q.window = 0;
+    return q;
+}
+
 int64_t tllm_paged_attention_workspace(const tllm_paged_attention_params_t* p)
 {
     int64_t bytes = -1;
     if (guarded([&] {
             if (!attention_fits(p))
                 return true;
-            bytes = p->n_rows ? (int64_t) paged_attention_workspace(*p) : 0;
+            bytes = p->n_rows ? (int64_t) paged_attention_workspace(as_launched(*p)) : 0;
             return false;
         }))
         return -1;
@@ -178,12 +187,13 @@ int32_t tllm_paged_attention(const tllm_paged_attention_params_t* p, void* works
             return true;
         if (p->n_rows == 0)
             return false;
-        if (paged_attention_workspace(*p) && (!workspace || !aligned(workspace, 16)))
+        const tllm_paged_attention_params_t q = as_launched(*p);
+        if (paged_attention_workspace(q) && (!workspace || !aligned(workspace, 16)))
         {
             set_error("tllm_paged_attention: the workspace is null or not 16-byte aligned");
             return true;
         }
-        return launch_paged_attention(*p, workspace, reinterpret_cast<hipStream_t>(stream)) != 0;
+        return launch_paged_attention(q, workspace, reinterpret_cast<hipStream_t>(stream)) != 0;
     });
 }
 
