@@ -33,7 +33,7 @@ extern "C" {
  *   cu_tokens     [n_seqs + 1] the packed rows of request b are cu_tokens[b] .. cu_tokens[b + 1];
  *   slot_map      [n_rows] block * page_size + offset of each row's token, -1 behind the last row;
  *   positions     [n_rows] its position in its request, -1 behind the last row;
- *   lens_out, ring_state_out: the state behind the step; they may be lens and ring_state themselves;
+ *   lens_out, ring_state_out: the state behind the step; they may be lens and ring_state themselves (no other two tensors may overlap);
  *   status        [1] 0, or a sum of 1: a request needs more than max_blocks pages, 2: the ring has too few blocks, 4: the step has more than
  *                 n_rows tokens, 8: a negative length, or a ring_state that cannot be (or would hold more than num_blocks).  A step
  *                 with a status changes no table, ring or state, and has no rows: cu_tokens is 0, every slot -1.
@@ -106,6 +106,7 @@ int32_t tllm_paged_append(const tllm_paged_append_params_t* p, tllm_stream_t str
  *   max_new  no request has more rows (rows behind that many are not computed);
  *   max_kv   an expectation of the longest kv_lens, for how the work is split; any kv_lens up to max_blocks * page_size is right.
  * Table entries that are no block of the pool count as masked.  Lengths beyond the table are cut to it.
+ * out may be q itself, with its strides.
  * Workspace: tllm_paged_attention_workspace() bytes, 16-byte aligned, not shared by calls that may overlap.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct
@@ -134,7 +135,7 @@ int32_t tllm_paged_attention(const tllm_paged_attention_params_t* p, void* works
  *   packed  [ceil(N / 16)][ceil(K / 128)][64][16] bytes: lane l = 16 g + r of a tile holds, in its 32-bit word j, row r's eight
  *           elements k = 32 j + 8 g + e of the tile, as nibbles q + 8 in the order e = 0 2 4 6 1 3 5 7; padding is 8 (zero);
  *   scales  [ceil(K / group)][16 * ceil(N / 16)], padding 0.
- * x rows start 16-byte aligned (ldx a multiple of 8); y rows 2-byte aligned.
+ * x rows start 16-byte aligned (ldx a multiple of 8); y rows 2-byte aligned; y does not overlap x.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct
 {

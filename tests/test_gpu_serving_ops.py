@@ -616,6 +616,33 @@ def test_two_streams_at_once():
 
 
 # ------------------------------------------------------------------------------------------------ refusals
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+@pytest.mark.parametrize('spans', [[(0, 5), (70, 1), (300, 2)], [(100, 300), (9, 1)], [(9000, 1)], [(9000, 100)]], ids=['few', 'prompt', 'split', 'split prompt'])
+def test_attention_in_place_of_its_queries(spans, dtype):
+    """out is q, both a view into a packed projection: the bits are those of the call with a result of its own."""
+    torch.manual_seed(5)
+    pages = [-(-(past + new) // 64) for past, new in spans]
+    cache = P.PagedKV8Cache(torch.randint(-127, 128, (sum(pages), 2, 2, 64 * 128), dtype=torch.int8, device='cuda'), torch.rand((sum(pages), 2, 2), device='cuda') * 1e-2, 64, 128)
+    table = torch.zeros((len(spans), max(pages)), dtype=torch.int32, device='cuda')
+    ids = torch.randperm(sum(pages), dtype=torch.int32, device='cuda')
+    for b, n in enumerate(pages):
+        table[b, :n] = ids[sum(pages[:b]):sum(pages[:b + 1])]
+    rows = [new for _, new in spans]
+    qkv = torch.randn((sum(rows), 8, 128), device='cuda').to(TYPES[dtype])
+    q, kept = qkv[:, :6], qkv.clone()
+    args = table, gpu(np.cumsum([0] + rows)), gpu([past + new for past, new in spans]), max(rows)
+    want = cache.attention(q, *args)
+    assert cache.attention(q, *args, out=q) is q
+    assert torch.equal(q, want) and torch.equal(qkv[:, 6:], kept[:, 6:])
+
+
+def test_tensors_of_the_objects_stay():
+    cache, mm, plan = P.PagedKV8Cache.empty(2, 16, 1, 64), G.GroupQuantMatmul(torch.zeros((1, 32), dtype=torch.int8, device='cuda'), torch.ones((1, 1), device='cuda').half(), 32), P.StepPlan(1, 1)
+    for thing, name in ((cache, 'pool'), (cache, 'scales'), (mm, 'scales'), (mm, 'packed'), (plan, 'lens'), (plan, 'slot_map')):
+        with pytest.raises(AttributeError, match='stays'):
+            setattr(thing, name, getattr(thing, name).clone())
+
+
 def test_wrappers_refuse():
     c = P.PagedKV8Cache.empty(4, 16, 2, 64)
     k = torch.zeros(3, 2, 64, dtype=torch.float16, device='cuda')

@@ -90,6 +90,17 @@ def test_plan_refuses():
         refused(call, p, word, **bad)
 
 
+def test_plan_refuses_results_on_other_tensors():
+    lib = P._lib()
+    call = lambda p: lib.tllm_paged_plan(ctypes.addressof(p), None)
+    p = plan_params()
+    for i, (n, _) in enumerate(p._fields_[6:]):
+        setattr(p, n, AT * (i + 1))
+    for bad in (dict(lens_out=p.new_lens), dict(lens_out=p.lens + 4), dict(ring_state_out=p.ring_state + 4), dict(cu_tokens=p.lens), dict(slot_map=p.positions), dict(status=p.cu_tokens + 16),
+                dict(positions=p.ring + 396), dict(lens_out=p.ring_state), dict(ring_state_out=p.lens)):
+        refused(call, p, 'lies where', **bad)
+
+
 def append_params():
     p = AppendParams(8, 2, 4, 64, 16, 100, capi.HALF, capi.INT8, 64, 0, 50)
     for n, t in p._fields_:
@@ -131,7 +142,7 @@ def test_attention_refuses():
                       ('dtype', dict(dtype=capi.INT8)), ('cache_type', dict(cache_type=capi.UINT8)), ('max_new', dict(max_new=0)), ('max_kv', dict(max_kv=-1)), ('window', dict(window=-1)),
                       ('scale', dict(scale=float('nan'))), ('scale', dict(scale=float('inf'))), ('null', dict(block_table=None)), ('null', dict(cu_tokens=None)), ('aligned', dict(kv_lens=AT + 1)),
                       ('q has', dict(q=AT + 2)), ('q has', dict(q_row=63)), ('out has', dict(out_head=9)), ('null out', dict(out=None)),
-                      ('one launch', dict(n_seqs=4096, max_new=1 << 19))):
+                      ('one launch', dict(n_seqs=4096, max_new=1 << 19, n_rows=1 << 19))):
         refused(call, p, word, **bad)
     assert lib.tllm_paged_attention_workspace(None) == -1
     p.max_new = 0
@@ -144,7 +155,7 @@ def test_matmul_refuses():
     p = MatmulParams(2, 10, 64, 32, capi.HALF, 64, 10, AT, AT, AT, AT)
     for word, bad in (('dtype', dict(dtype=capi.FLOAT)), ('group', dict(group=16)), ('rows', dict(rows=-1)), ('k 48', dict(k=48)), ('k 0', dict(k=0)), ('n 0', dict(n=0)),
                       ('weights', dict(packed=None)), ('weights', dict(packed=AT + 8)), ('scales', dict(scales=AT + 2)), ('x has', dict(x=AT + 2)), ('x has', dict(ldx=63)), ('x has', dict(ldx=32)),
-                      ('y is', dict(y=None)), ('y is', dict(ldy=9))):
+                      ('y is', dict(y=None)), ('y is', dict(ldy=9)), ('y lies', dict())):
         refused(call, p, word, **bad)
 
 
@@ -172,6 +183,30 @@ def test_packing_refuses():
             G.pack(*bad)
     with pytest.raises(ValueError):
         G.GroupQuantMatmul(q, s, 32)  # not on a GPU
+
+
+def test_quantize():
+    w = torch.linspace(-3, 3, 5 * 96).view(5, 96)
+    w[1] = 0
+    q, s = G.quantize(torch.nn.Parameter(w), 64)
+    assert q.shape == (5, 96) and s.shape == (5, 2) and not s.requires_grad and int(q.min()) >= -8 and int(q.max()) <= 7 and (s[1] == 1).all() and (q[1] == 0).all()
+    # half a step, and what the scale's rounding (2^-11) moves 7 steps by
+    assert ((q.float() * s.float().repeat_interleave(64, 1)[:, :96] - w).abs() <= (0.5 + 7 * 2.0**-11) * s.float().repeat_interleave(64, 1)[:, :96]).all()
+    for bad in (float('inf'), float('nan'), 1e6):
+        x = w.clone()
+        x[2, 70] = bad
+        with pytest.raises(ValueError, match='finite'):
+            G.quantize(x, 64)
+
+
+def test_public_names():
+    import tensorrt_llm.quantization as Q
+    import tensorrt_llm.runtime as R
+    assert Q.GroupQuantMatmul is G.GroupQuantMatmul and R.PagedKV8Cache is P.PagedKV8Cache and R.plan_step is P.plan_step and R.StepPlan is P.StepPlan
+    assert R.DeviceBlockPool is P.DeviceBlockPool and R.rope_table is P.rope_table
+    for module in (Q, R):
+        with pytest.raises(AttributeError):
+            module.no_such_name
 
 
 def test_caches_and_pools_refuse():

@@ -1,6 +1,7 @@
 // extern "C" surface of include/tllm_serving_api.h: every size, type, stride and alignment that a kernel relies on is checked here, on the host,
 // before anything is launched.  What only the device knows (lengths, table entries, slots) the kernels check themselves.
 #include "../kernels/serving_kernels.h"
+#include <algorithm>
 #include <exception>
 #include <initializer_list>
 
@@ -22,6 +23,18 @@ bool is_head(int32_t v)
 bool aligned(const void* p, size_t to)
 {
     return reinterpret_cast<uintptr_t>(p) % to == 0;
+}
+
+struct Range
+{
+    const void* at;
+    int64_t bytes;
+};
+
+bool overlap(const Range& a, const Range& b)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
 }
 
 constexpr int32_t kMaxRows = 1 << 19, kMaxHeads = 1024;
@@ -52,6 +65,18 @@ bool plan_fits(const tllm_paged_plan_params_t* p)
     for (const void* t : std::initializer_list<const void*>{p->lens, p->new_lens, p->ring, p->ring_state, p->block_table, p->cu_tokens, p->slot_map, p->positions, p->lens_out,
              p->ring_state_out, p->status})
         TLLM_REFUSE(!aligned(t, 4), "%s: a tensor is not 4-byte aligned", me);
+    // several workgroups read what one of them writes, unless it is the whole of the same state
+    const int64_t n = p->n_seqs * 4, rows = p->n_rows * 4;
+    const Range reads[] = {{p->lens, n}, {p->new_lens, n}, {p->ring_state, 8}, {p->ring, (int64_t) p->num_blocks * 4}};
+    const Range writes[] = {{p->lens_out, n}, {p->ring_state_out, 8}, {p->cu_tokens, n + 4}, {p->slot_map, rows}, {p->positions, rows}, {p->status, 4}};
+    for (const Range& w : writes)
+    {
+        for (const Range& r : reads)
+            TLLM_REFUSE(overlap(w, r) && !(w.at == r.at && ((w.at == p->lens_out && r.at == p->lens) || (w.at == p->ring_state_out && r.at == p->ring_state))),
+                "%s: a result lies where another tensor does", me);
+        for (const Range& o : writes)
+            TLLM_REFUSE(&o != &w && overlap(w, o), "%s: a result lies where another tensor does", me);
+    }
     return true;
 }
 
@@ -111,9 +136,10 @@ bool attention_fits(const tllm_paged_attention_params_t* p)
     TLLM_REFUSE(!(p->scale >= 0.f && p->scale < 1e30f), "%s: the scale is negative or not finite", me);
     TLLM_REFUSE(!p->block_table || !p->cu_tokens || !p->kv_lens || !aligned(p->block_table, 4) || !aligned(p->cu_tokens, 4) || !aligned(p->kv_lens, 4),
         "%s: tables and lengths are null or not 4-byte aligned", me);
-    TLLM_REFUSE((int64_t) p->n_seqs * p->kv_heads * (((int64_t) p->max_new * (p->q_heads / p->kv_heads) + 15) / 16) > INT32_MAX / 64 - 8
-            || (int64_t) p->n_seqs * p->max_new * p->q_heads > INT32_MAX,
-        "%s: %d requests of up to %d rows are more than one launch takes", me, p->n_seqs, p->max_new);
+    const int64_t max_new = std::min(p->max_new, p->n_rows);
+    TLLM_REFUSE((int64_t) p->n_seqs * p->kv_heads * ((max_new * (p->q_heads / p->kv_heads) + 15) / 16) > INT32_MAX / 64 - 8
+            || p->n_seqs * max_new * p->q_heads > INT32_MAX,
+        "%s: %d requests of up to %lld rows are more than one launch takes", me, p->n_seqs, (long long) max_new);
     return p->n_rows == 0 || (rows_fit(me, "q", p->q, p->q_row, p->q_head) && rows_fit(me, "out", p->out, p->out_row, p->out_head));
 }
 
@@ -128,6 +154,7 @@ bool matmul_fits(const tllm_group_matmul_params_t* p)
     TLLM_REFUSE(!p->packed || !aligned(p->packed, 16) || !p->scales || !aligned(p->scales, 16), "%s: weights or scales are null or not 16-byte aligned", me);
     TLLM_REFUSE(p->rows && (!p->x || !aligned(p->x, 16) || p->ldx % 8 || (p->rows > 1 && p->ldx < p->k)), "%s: x has to be 16-byte aligned with a row stride that is a multiple of 8, at least k", me);
     TLLM_REFUSE(p->rows && (!p->y || !aligned(p->y, 2) || (p->rows > 1 && p->ldy < p->n)), "%s: y is null, not 2-byte aligned or its row stride is less than n", me);
+    TLLM_REFUSE(p->rows && p->x == p->y, "%s: y lies where x does", me);
     return true;
 }
 
@@ -158,12 +185,13 @@ int32_t tllm_paged_append(const tllm_paged_append_params_t* p, tllm_stream_t str
     return guarded([&] { return !append_fits(p) || (p->n_rows && launch_paged_append(*p, reinterpret_cast<hipStream_t>(stream))); });
 }
 
-// what the kernels get: a window that no row can fill is none (and does not take positions out of range)
+// what the kernels get: a window that no row can fill is none (and does not take positions out of range), no request has more rows than there are
 static tllm_paged_attention_params_t as_launched(const tllm_paged_attention_params_t& p)
 {
     tllm_paged_attention_params_t q = p;
     if (q.window >= (int64_t) q.max_blocks * q.page_size)
         q.window = 0;
+    q.max_new = std::min(q.max_new, q.n_rows);
     return q;
 }
 

@@ -8,7 +8,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..plugin import capi
-from ..runtime.paged_kv8 import on_device
+from ..runtime.paged_kv8 import Fixed, on_device
 
 GROUPS = (32, 64, 128)
 _ACT = {torch.float16: capi.HALF, torch.bfloat16: 7}
@@ -36,15 +36,17 @@ def _checked(n: int, k: int, group: int):
 
 
 def quantize(weight: torch.Tensor, group: int, dtype=torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
-    """weight [n, k] -> (q int8 [n, k] in -7 .. 7, scales `dtype` [n, ceil(k / group)]): the scale is the group's largest magnitude / 7 rounded to
+    """weight [n, k] -> (q int8 [n, k] in -8 .. 7, scales `dtype` [n, ceil(k / group)]): the scale is the group's largest magnitude / 7 rounded to
     `dtype` (1 for a group of zeros, and for one whose scale would round to 0), q the nearest even of weight / scale."""
     n, k = weight.shape
     _checked(n, k, group)
     count = -(-k // group)
     w = torch.zeros((n, count * group), dtype=torch.float32, device=weight.device)
-    w[:, :k] = weight
+    w[:, :k] = weight.detach()
     w = w.view(n, count, group)
     scales = (w.abs().amax(-1) / 7).to(dtype)
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError(f'the weights have a group whose scale is not finite in {dtype}')
     scales = torch.where(scales == 0, torch.ones_like(scales), scales)
     q = torch.round(w / scales.float()[..., None]).clamp_(-8, 7).to(torch.int8)
     return q.view(n, -1)[:, :k].contiguous(), scales
@@ -59,6 +61,7 @@ def pack(q: torch.Tensor, scales: torch.Tensor, group: int) -> Tuple[torch.Tenso
                          f'{scales.dtype} {tuple(scales.shape)}')
     if int(q.min()) < -8 or int(q.max()) > 7:
         raise ValueError('q has values outside -8 .. 7')
+    scales = scales.detach()
     tiles, steps = -(-n // 16), -(-k // 128)
     u = torch.full((16 * tiles, 128 * steps), 8, dtype=torch.uint8, device=q.device)
     u[:n, :k] = (q + 8).to(torch.uint8)
@@ -69,7 +72,7 @@ def pack(q: torch.Tensor, scales: torch.Tensor, group: int) -> Tuple[torch.Tenso
     return u.reshape(tiles, steps, 64, 16).contiguous(), s
 
 
-class GroupQuantMatmul(object):
+class GroupQuantMatmul(Fixed):
     """y = x W^T with W packed once: q int8 [n, k] in -8 .. 7, scales float16 or bfloat16 [n, ceil(k / group)], which is the type of x and y too."""
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, group: int):
@@ -84,7 +87,7 @@ class GroupQuantMatmul(object):
         return cls(*quantize(weight, group, dtype), group)
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """x [.., k] -> [.., n]; a two-dimensional x may have strided rows.  `out` [rows, n] takes the result if given."""
+        """x [.., k] -> [.., n]; a two-dimensional x may have strided rows.  `out` [rows, n] takes the result if given; it does not overlap x."""
         index, n, k = self._index, self.n, self.k
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         (rows, wide), (row, one) = x2.shape, x2.stride()

@@ -86,7 +86,17 @@ def _rows(what, t, rows, heads, size, dtype, index, written=False):
                      f'{", no two rows on one place," if written else ""} on GPU {index}: {_got(t)}')
 
 
-class StepPlan(object):
+class Fixed(object):
+    """Attributes are set once: calls use the tensors that were checked, and do not check them again."""
+    __slots__ = ()
+
+    def __setattr__(self, name, value):
+        if hasattr(self, name):
+            raise AttributeError(f'{name} of a {type(self).__name__} stays what it is: make another one')
+        object.__setattr__(self, name, value)
+
+
+class StepPlan(Fixed):
     """What a step needs to know of its pages, in tensors that are written anew by every plan: cu_tokens [n_seqs + 1], slot_map and positions [n_rows]
     (-1 behind the last row), lens [n_seqs] and ring_state [2] behind the step, status [1] (0: fine; tllm_serving_api.h has the others).  The tensors
     stay the same ones for the plan's life."""
@@ -98,11 +108,8 @@ class StepPlan(object):
         index = cu.get_device()
         lens, ring_state = new(n_seqs) if lens is None else lens, new(2) if ring_state is None else ring_state
         at = (cu.data_ptr(), slots.data_ptr(), places.data_ptr(), _ints('lens', lens, n_seqs, index), _ints('ring_state', ring_state, 2, index), status.data_ptr())
-        for name, v in dict(n_seqs=n_seqs, n_rows=n_rows, index=index, cu_tokens=cu, slot_map=slots, positions=places, status=status, lens=lens, ring_state=ring_state, _at=at).items():
-            object.__setattr__(self, name, v)
-
-    def __setattr__(self, name, value):
-        raise AttributeError('the tensors of a StepPlan are its own: make another one')
+        self.n_seqs, self.n_rows, self.index, self.cu_tokens, self.slot_map, self.positions, self.status, self.lens, self.ring_state, self._at = (
+            n_seqs, n_rows, index, cu, slots, places, status, lens, ring_state, at)
 
 
 def plan_step(lens: torch.Tensor, new_lens: torch.Tensor, ring: torch.Tensor, ring_state: torch.Tensor, block_table: torch.Tensor, page_size: int,
@@ -156,7 +163,7 @@ def rope_table(positions: int, rot_dim: int, base: float = 10000.0, factor: floa
     return torch.stack([angle.cos(), angle.sin()], -1).to(torch.float32).to(device)
 
 
-class PagedKV8Cache(object):
+class PagedKV8Cache(Fixed):
     """One layer's cache: `pool` int8 or float8_e4m3fn [blocks, 2, kv_heads, page_size * head_size] (keys of a page and head [page_size, head_size],
     values [head_size, page_size]) and `scales` fp32 [blocks, 2, kv_heads].  The tensors are the caller's, the same ones for the cache's life;
     `PagedKV8Cache.empty` makes them."""
@@ -218,7 +225,7 @@ class PagedKV8Cache(object):
         """softmax(scale q k) v of q [rows, heads, head_size] over the cached keys of each request, causal, the last `window` keys only if window > 0.
         Request b has the rows cu_tokens[b] .. cu_tokens[b + 1] and kv_lens[b] cached tokens, its rows the last of them.  `max_new`: no request has more
         rows; `max_kv`: the longest length to expect (default: what the tables hold), which only says how the work is split.  scale: 1 / sqrt(head_size)
-        unless given.  Rows that belong to no request are left as `out` had them (a new tensor's are undefined)."""
+        unless given; `out` may be q.  Rows that belong to no request are left as `out` had them (a new tensor's are undefined)."""
         index, size, dtype, rows, n = self._index, self.head_size, q.dtype, q.shape[0], kv_lens.numel()
         act = _ACT.get(dtype)
         if act is None:
