@@ -384,6 +384,14 @@ def test_attention_prompts_split_over_workgroups(window, kind, dtype, size):
     check_attention(np.random.default_rng(size), kind, dtype, 64, size, 1, 2, [(5000, 40), (3100, 1), (0, 0), (70, 30), (9, 20)], window=window, max_kv=9000, spare_rows=1)
 
 
+@pytest.mark.parametrize('kind,dtype,size', [('int8', 'fp16', 128), ('fp8', 'bf16', 64), ('int8', 'bf16', 256)])
+@pytest.mark.parametrize('kv,group', [(2, 1), (1, 4), (1, 20)])
+@pytest.mark.parametrize('window', [0, 2200])
+@pytest.mark.parametrize('spans', [[(4200, 1), (0, 100), (2500, 3), (70, 1), (0, 0), (2100, 40)], [(4200, 1), (3100, 30)]], ids=['many', 'two'])
+def test_attention_of_tokens_beside_prompts(spans, window, kv, group, kind, dtype, size):
+    check_attention(np.random.default_rng(len(spans) + window), kind, dtype, 64, size, kv, group, spans, window=window, spare_rows=3)
+
+
 def test_attention_rows_that_see_nothing():
     """More rows than cached tokens: the first ones stand before the cache's beginning.  Lengths below zero and beyond the table."""
     rng = np.random.default_rng(8)

@@ -164,11 +164,14 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b)
         return (uint32_t) f2h(a) | (uint32_t) f2h(b) << 16;
 }
 
+// The keys of a row in parts, each by its own workgroup.
 struct Split
 {
-    float* o;  // [n_rows][q_heads][parts][DIM], not divided by l
-    float* ml; // [n_rows][q_heads][parts][2]
+    float* o;  // [rows][q_heads][parts][DIM], not divided by l
+    float* ml; // [rows][q_heads][parts][2]
     int parts;
+    int per; // rows a request has in these, 0: they are the batch's rows
+    __device__ __forceinline__ int64_t at(int b, int row0, int i, int heads, int h) const { return ((int64_t) ((per ? b * per : row0) + i) * heads + h) * parts; }
 };
 
 // The value scales: the reference that O is in units of, and what a tile's pages say to a lane.
@@ -429,7 +432,7 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
         const int utoken = urow / group, uh = head * group + urow - utoken * group;
         if (split.parts > 1)
         {
-            const int64_t at = ((int64_t) (req.row0 + utoken) * p.q_heads + uh) * split.parts + part;
+            const int64_t at = split.at(b, req.row0, utoken, p.q_heads, uh) + part;
             *reinterpret_cast<f32x4*>(split.o + at * DIM + d) = a;
             if (d == 0)
             {
@@ -468,9 +471,11 @@ struct TileForm
     static constexpr int kBuffers = DIM == 256 ? 1 : 2, kLds = kBuffers * kFrags * 1024;
 };
 
-// Tiles of kRows rows of a request and key head.  Requests of at most 16 rows in the same batch take rows_body.
+// Tiles of kRows rows of a request and key head.  Requests of at most 16 rows in the same batch take rows_body, in the first light_groups workgroups,
+// or in those of their tile 0 if there are none.
 template <int DIM, bool BF16, bool FP8>
-__global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm_paged_attention_params_t p, const int shift, const int row_tiles, const Split split)
+__global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm_paged_attention_params_t p, const int shift, const int row_tiles, const int light_groups, const Split light,
+    const Split split)
 {
     using F = TileForm<DIM>;
     constexpr int kSteps = DIM / 32, kOut = DIM / 16, RT = F::kRt;
@@ -478,8 +483,9 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
     // Workgroups go round the XCDs: the row tiles of one request and head follow each other on one XCD, whose L2 holds their keys.  Those with the
     // most keys first, and the other way round where a pair of request and head begins in an odd 32: workgroups 32 apart of an XCD meet on
     // one CU (2048 tokens behind 1500, 32 heads of 128: 125 us, 148 without)
-    const int xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, order = at8 % row_tiles, pair = at8 / row_tiles * 8 + xcd;
-    const int tile = (at8 - order) >> 5 & 1 ? order : row_tiles - 1 - order, part = blockIdx.y;
+    const int id = blockIdx.x - light_groups, xcd = id & 7, at8 = id >> 3, order = at8 % row_tiles;
+    const int tile = id < 0 ? 0 : (at8 - order) >> 5 & 1 ? order : row_tiles - 1 - order;
+    const int part = id < 0 ? blockIdx.x % light.parts : blockIdx.y, pair = id < 0 ? blockIdx.x / light.parts : at8 / row_tiles * 8 + xcd;
     if (pair >= p.n_seqs * p.kv_heads)
         return;
     const int head = pair % p.kv_heads, b = pair / p.kv_heads, group = p.q_heads / p.kv_heads;
@@ -488,7 +494,13 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
     if (tile * F::kRows >= rows)
         return;
     if (rows <= 16)
-        return rows_body<DIM, BF16, FP8, 4>(p, shift, split, req, head, b, 0, part, reinterpret_cast<float*>(frags));
+    {
+        if (blockIdx.y == 0 && (id < 0 || light_groups == 0))
+            rows_body<DIM, BF16, FP8, 4>(p, shift, light, req, head, b, 0, part, reinterpret_cast<float*>(frags));
+        return;
+    }
+    if (id < 0)
+        return;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int first = req.len - req.rows;
@@ -684,7 +696,7 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
         const float unit = ref.v * __builtin_amdgcn_exp2f(-kPShift);
         if (split.parts > 1)
         {
-            const int64_t at = ((int64_t) (req.row0 + token) * p.q_heads + qh) * split.parts + part;
+            const int64_t at = split.at(b, req.row0, token, p.q_heads, qh) + part;
 #pragma unroll
             for (int d = 0; d < kOut; ++d)
                 *reinterpret_cast<f32x4*>(split.o + at * DIM + 16 * d + 4 * g) = o[n][d] * unit;
@@ -703,9 +715,9 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
     }
 }
 
-// Parts of the keys -> rows: a workgroup per row and head, its waves take the parts in turn.
+// Parts of the keys -> rows: a workgroup per row and head, `per` rows a request; its waves take the parts in turn.
 template <int DIM, bool BF16>
-__global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_params_t p, const int shift, const Split split)
+__global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_params_t p, const int shift, const int per, const Split light, const Split heavy)
 {
     constexpr int kPer = DIM / 64;
     __shared__ float os[4][DIM];
@@ -713,11 +725,12 @@ __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_p
     int id = blockIdx.x;
     const int h = id % p.q_heads;
     id /= p.q_heads;
-    const int i = id % p.max_new, b = id / p.max_new;
+    const int i = id % per, b = id / per;
     const Request req = request_of(p, b, shift);
-    if (i >= req.rows)
+    const Split split = min(req.rows, p.max_new) * (p.q_heads / p.kv_heads) <= 16 ? light : heavy;
+    if (i >= req.rows || split.parts == 1)
         return;
-    const int64_t at = ((int64_t) (req.row0 + i) * p.q_heads + h) * split.parts;
+    const int64_t at = split.at(b, req.row0, i, p.q_heads, h);
     float m = -INFINITY, l = 0.f; // of part `lane`: there are 64 at most
     if (lane < split.parts)
     {
@@ -773,24 +786,39 @@ int row_tiles_of(const tllm_paged_attention_params_t& p) // of tile_kernel
 // Workgroups that the keys are split into.
 // Requests of one tile of rows: with fewer requests and key heads than CUs two a CU.  With more of them the split only evens out contexts of
 // different lengths, and joining costs more than that unless they are long (64 x 8 heads over 300 to 600 keys of 128: 21 us whole, 28 in
-// two parts; 48 x 8 over 4000 to 8000: 115 in three, 126 whole; one of 32 heads over 1032: 10.7 in 8 parts, 12.4 in 4).
+// two parts; 48 x 8 over 4000 to 8000: 115 in three, 126 whole; one of 32 heads over 1032: 10.7 in 8 parts, 12.4 in 4).  The host does not know
+// how many such requests there are among prompts: at most as many as leave the others no more than max_new rows each (4 tokens over 30000 keys beside a prompt of 1024, 32 heads
+// on 8: 76 us, 338 with their keys whole; tokens alone 44, the prompt alone 36).
 // More rows: what fills two places on every CU, where their tiles do not (443 tokens of one head over 57000 keys: 7 tiles).
-int parts_of(const tllm_paged_attention_params_t& p)
+struct Parts
+{
+    int light, heavy, per; // of requests of one tile of rows, of the others; rows that one of the light ones has at most
+};
+Parts parts_of(const tllm_paged_attention_params_t& p)
 {
     const int64_t pairs = (int64_t) p.n_seqs * p.kv_heads, cus = launch_util::device_cus();
     const int64_t keys = p.window > 0 ? std::min<int64_t>((int64_t) p.window + p.max_new, p.max_kv) : p.max_kv;
-    int64_t want, least;
-    if (one_tile(p))
+    auto within = [](int64_t want, int64_t most) { return (int) std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64)); };
+    Parts s = {1, 1, std::min(p.max_new, 16 / (p.q_heads / p.kv_heads))};
+    int64_t few = pairs, least = pairs >= cus ? 2048 : pairs * 4 >= cus ? 512 : 128;
+    if (!one_tile(p))
     {
-        want = ((pairs < cus ? 2 : 4) * cus + pairs - 1) / pairs;
-        least = pairs >= cus ? 2048 : pairs * 4 >= cus ? 512 : 128;
-    }
-    else
-    {
-        want = 2 * cus / (pairs * row_tiles_of(p));
+        s.heavy = within(2 * cus / (pairs * row_tiles_of(p)), keys / 1024);
+        few = s.per ? std::min<int64_t>(p.n_seqs - 1, ((int64_t) p.n_seqs * p.max_new - p.n_rows) / (p.max_new - s.per)) * p.kv_heads : 0;
         least = 1024;
     }
-    return (int) std::max<int64_t>(1, std::min<int64_t>(std::min(want, keys / least), 64));
+    if (few > 0)
+        s.light = within(((few < cus ? 2 : 4) * cus + few - 1) / few, keys / least);
+    return s;
+}
+
+struct Places // rows of the workspace
+{
+    int64_t light, heavy;
+};
+Places places_of(const tllm_paged_attention_params_t& p, const Parts& s)
+{
+    return {s.light > 1 ? (int64_t) p.n_seqs * s.per * p.q_heads * s.light : 0, s.heavy > 1 ? (int64_t) p.n_rows * p.q_heads * s.heavy : 0};
 }
 
 template <int DIM, bool BF16, bool FP8>
@@ -798,21 +826,24 @@ void launch_form(const tllm_paged_attention_params_t& p, void* workspace, hipStr
 {
     const int shift = __builtin_ctz((unsigned) p.page_size);
     const int64_t pairs = (int64_t) p.n_seqs * p.kv_heads;
-    const int parts = parts_of(p);
-    Split split = {static_cast<float*>(workspace), nullptr, parts};
-    if (parts > 1)
-        split.ml = split.o + (int64_t) p.n_rows * p.q_heads * parts * DIM;
+    const Parts s = parts_of(p);
+    const auto n = places_of(p, s);
+    float* const o = static_cast<float*>(workspace);
+    float* const ml = o + (n.light + n.heavy) * DIM;
+    const Split light = {o, ml, s.light, s.per}, heavy = {o + n.light * DIM, ml + n.light * 2, s.heavy, 0};
     if (one_tile(p))
-        rows_kernel<DIM, BF16, FP8, 4><<<(unsigned) (pairs * parts), 256, 0, stream>>>(p, shift, split);
+        rows_kernel<DIM, BF16, FP8, 4><<<(unsigned) (pairs * s.light), 256, 0, stream>>>(p, shift, light);
     else
     {
         using F = TileForm<DIM>;
-        const int row_tiles = row_tiles_of(p);
+        const int row_tiles = row_tiles_of(p), light_groups = s.light > 1 ? (int) ((pairs * s.light + 7) / 8 * 8) : 0;
         launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&tile_kernel<DIM, BF16, FP8>), F::kLds);
-        tile_kernel<DIM, BF16, FP8><<<dim3((unsigned) ((pairs + 7) / 8 * 8 * row_tiles), parts), 256, F::kLds, stream>>>(p, shift, row_tiles, split);
+        tile_kernel<DIM, BF16, FP8>
+            <<<dim3((unsigned) (light_groups + (pairs + 7) / 8 * 8 * row_tiles), s.heavy), 256, F::kLds, stream>>>(p, shift, row_tiles, light_groups, light, heavy);
     }
-    if (parts > 1)
-        merge_kernel<DIM, BF16><<<(unsigned) ((int64_t) p.n_seqs * p.max_new * p.q_heads), 256, 0, stream>>>(p, shift, split);
+    const int per = s.heavy > 1 ? p.max_new : s.per;
+    if (s.light > 1 || s.heavy > 1)
+        merge_kernel<DIM, BF16><<<(unsigned) ((int64_t) p.n_seqs * per * p.q_heads), 256, 0, stream>>>(p, shift, per, light, heavy);
 }
 
 template <int DIM, bool BF16>
@@ -827,8 +858,8 @@ void launch_dim(const tllm_paged_attention_params_t& p, void* workspace, hipStre
 
 size_t paged_attention_workspace(const tllm_paged_attention_params_t& p)
 {
-    const int parts = parts_of(p);
-    return parts > 1 ? (size_t) p.n_rows * p.q_heads * parts * (p.head_size + 2) * 4 : 0;
+    const Places n = places_of(p, parts_of(p));
+    return (size_t) (n.light + n.heavy) * (p.head_size + 2) * 4;
 }
 
 int launch_paged_attention(const tllm_paged_attention_params_t& p, void* workspace, hipStream_t stream)
