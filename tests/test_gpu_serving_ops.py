@@ -472,13 +472,13 @@ def check_product(rng, rows, n, k, group, dtype, strided=False):
 @pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
 @pytest.mark.parametrize('group', [32, 64, 128])
 @pytest.mark.parametrize('rows,n,k', [(1, 16, 32), (1, 1, 128), (1, 4096, 4096), (3, 100, 160), (16, 257, 992), (17, 64, 1024), (32, 130, 96), (33, 513, 2080), (64, 96, 11008),
-                                      (65, 200, 256), (130, 300, 640), (257, 1000, 1312), (700, 31, 224)])
+                                      (65, 200, 256), (130, 300, 640), (257, 1000, 1312), (700, 31, 224), (1, 4097, 4128), (5, 2050, 1056)])
 def test_group_matmul(rows, n, k, group, dtype):
     check_product(np.random.default_rng(rows + n + k), rows, n, k, group, dtype)
 
 
 @pytest.mark.parametrize('group,dtype', [(128, 'fp16'), (32, 'bf16'), (64, 'fp16')])
-@pytest.mark.parametrize('rows,n', [(1, 1), (1, 4116), (1, 8195), (1, 12295), (1027, 1), (5, 4111), (5, 8207), (5, 12291), (1064, 17), (9, 4099), (17, 4118), (17, 6155), (1362, 65), (1381, 129), (17, 8196), (33, 6146), (1671, 130), (1633, 258), (33, 8197), (65, 6149), (129, 10943), (385, 12378)])
+@pytest.mark.parametrize('rows,n', [(1, 1), (1, 4116), (1, 8195), (1, 12295), (1027, 1), (5, 4111), (5, 8207), (5, 12291), (1064, 17), (9, 4099), (17, 4118), (17, 6155), (1362, 65), (1381, 129), (17, 8196), (33, 6146), (1671, 130), (1633, 258), (33, 8197), (65, 6149), (129, 10943), (385, 12378), (2054, 17), (33, 10883), (33, 12338), (259, 10913)])
 def test_group_matmul_in_every_form(rows, n, group, dtype):
     """Sizes at which each of the kernels' shapes is the quickest, k ending inside a tile."""
     check_product(np.random.default_rng(n), rows, n, 288, group, dtype)

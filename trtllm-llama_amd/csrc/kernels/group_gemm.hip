@@ -106,7 +106,7 @@ template <int R, int NT>
 struct FewForm
 {
     static constexpr int kSlot = R + NT + 1; // KB: x, weights, scales
-    static constexpr int kWaves = kSlot <= 4 ? 16 : kSlot <= 9 ? 8 : 4, kFit = 152 / (kWaves * kSlot), kDeep = kFit < 4 ? kFit : 4;
+    static constexpr int kWaves = kSlot <= 4 ? 16 : 8, kFit = 160 / (kWaves * kSlot), kDeep = kFit < 4 ? kFit : 4;
     static constexpr int kRing = kWaves * kDeep * kSlot * 1024, kMT = (R + 3) / 4;
     static_assert(kDeep >= 1 && kWaves * kMT * NT * 1024 <= 160 * 1024 && (kDeep - 1) * kSlot < 64, "the ring fits LDS and the counter");
     static constexpr int kLds = kRing > kWaves * kMT * NT * 1024 ? kRing : kWaves * kMT * NT * 1024;
@@ -255,50 +255,30 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(const tllm_group_matmul_pa
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     const uint32_t lds0 = (uint32_t) (uintptr_t) (lds_t*) lds;
 
-    // chunk c of a k-tile: x (row tile c / 4, k-step c % 4), then weights, then scales; a wave brings chunks wave, wave + 8, .. (the last one once
-    // more where they do not divide).  Each has an address that moves by the same step every k-tile.
-    const char* from[F::kPerWave];
-    uint32_t moves[F::kPerWave];
-    int k_of[F::kPerWave]; // of x: the lane's first k of the first tile, -1 for the others
+    // A wave brings k-step wave % 4 of row tiles wave / 4 + 2 i, and chunks wave, wave + 8, .. of the weights and then the scales (the last one
+    // once more where they do not divide).  Each has an address that moves by the same step every k-tile.
+    const int k0 = 32 * (wave & 3) + 8 * g;
+    const char* x_at[4];
 #pragma unroll
-    for (int i = 0; i < F::kPerWave; ++i)
-    {
-        const int c = min(i * 8 + wave, F::kChunks - 1);
-        k_of[i] = -1;
-        if (c < F::kX)
-        {
-            k_of[i] = 32 * (c & 3) + 8 * g;
-            from[i] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(p.x) + (int64_t) min((tile_m * 8 + (c >> 2)) * 16 + r, p.rows - 1) * p.ldx + k_of[i]);
-            moves[i] = 256;
-        }
-        else if (c < F::kX + F::kW)
-        {
-            from[i] = reinterpret_cast<const char*>(static_cast<const uint4*>(p.packed) + (int64_t) min(n0 + c - F::kX, n_tiles - 1) * k_tiles * 64 + lane);
-            moves[i] = 1024;
-        }
-        else
-        {
-            from[i] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(p.scales) + (int64_t) (c - F::kX - F::kW) * n_all + min(n0 * 16 + lane * 8, n_all - 8));
-            moves[i] = F::kGroups * n_all * 2;
-        }
-    }
+    for (int i = 0; i < 4; ++i)
+        x_at[i] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(p.x) + (int64_t) min((tile_m * 8 + 2 * i + wm) * 16 + r, p.rows - 1) * p.ldx + k0);
     auto bring = [&](int t) {
         const uint32_t to = lds0 + (t % kStages) * F::kStageBytes;
-        const bool tail = t == k_tiles - 1; // k may end inside: x is 0 there, as the weights are; a scale that is none is the last one's
+        const bool inside = t * 128 + k0 < p.k; // k may end inside the last k-tile: x is 0 there, as the weights are
 #pragma unroll
-        for (int i = 0; i < F::kPerWave; ++i)
+        for (int i = 0; i < 4; ++i)
         {
-            const int c = min(i * 8 + wave, F::kChunks - 1);
-            const void* at = from[i];
-            if (tail)
-            {
-                if (c < F::kX)
-                    at = t * 128 + k_of[i] < p.k ? at : kZeros;
-                else if (c >= F::kX + F::kW)
-                    at = from[i] - (int64_t) max(t * F::kGroups + c - F::kX - F::kW - (groups - 1), 0) * n_all * 2;
-            }
-            dma16(at, to + c * 1024);
-            from[i] += moves[i];
+            dma16(inside ? x_at[i] : reinterpret_cast<const char*>(kZeros), to + (i * 8 + wave) * 1024);
+            x_at[i] += 256;
+        }
+#pragma unroll
+        for (int i = 0; i < F::kPerWave - 4; ++i)
+        {
+            const int c = min(i * 8 + wave, F::kW + F::kGroups - 1);
+            const char* const at = c < F::kW
+                ? static_cast<const char*>(p.packed) + ((int64_t) min(n0 + c, n_tiles - 1) * k_tiles + t) * 1024
+                : static_cast<const char*>(p.scales) + (int64_t) min(t * F::kGroups + c - F::kW, groups - 1) * n_all * 2;
+            dma16(at + (c < F::kW ? lane * 16 : 2 * min(n0 * 16 + lane * 8, n_all - 8)), to + (F::kX + c) * 1024);
         }
     };
     f32x4 y[NT][4];
@@ -308,75 +288,96 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(const tllm_group_matmul_pa
         for (int j = 0; j < 4; ++j)
             y[i][j] = zero;
 
-    bring(0);
-    if (k_tiles > 1)
-        bring(1);
-    for (int t = 0; t < k_tiles; ++t)
-    {
-        // this k-tile has arrived (the next may be under way), for every wave, and the one before is read
+    auto arrived = [&](int t) { // k-tile t of what this wave has sent for, where t + 1 may be under way
         if (t + 1 < k_tiles)
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(F::kPerWave) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+    };
+    auto meet = [&] { // every wave; what this one has read of LDS is there
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    bring(0);
+    if (k_tiles > 1)
+        bring(1);
+    arrived(0);
+    meet();
+    if (wm)
+        meet();
+    for (int t = 0; t < k_tiles; ++t)
+    {
         if (t + 2 < k_tiles)
             bring(t + 2);
         const uint4* const at = lds + (t % kStages) * (F::kStageBytes / 16);
         const uint4* const xs = at + wm * 4 * 4 * 64 + lane;
         const uint4* const ws = at + (F::kX + wn * NT) * 64 + lane;
         const char* const ss = reinterpret_cast<const char*>(at + (F::kX + F::kW) * 64) + (wn * NT * 16 + 4 * g) * 2;
+        u32x4 words[NT], b[4][4];
+        uint2 scale[F::kGroups][NT];
 #pragma unroll
-        for (int q = 0; q < F::kGroups; ++q)
+        for (int n = 0; n < NT; ++n)
         {
-            u32x4 b[kSteps][4];
-            f32x4 sum[4];
+            words[n] = as_u32x4(ws[n * 64]);
+#pragma unroll
+            for (int q = 0; q < F::kGroups; ++q)
+                scale[q][n] = *reinterpret_cast<const uint2*>(ss + q * 1024 + n * 32);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                b[j][i] = as_u32x4(xs[(i * 4 + j) * 64]);
+        if (wm)
+            arrived(t + 1);
+        meet();
+        // Output tile n of group q is u = q NT + n: its products are under way while u + 1 is converted and u - 1 is scaled
+        constexpr int kUnits = F::kGroups * NT;
+        u32x4 w[2][kSteps];
+        f32x4 acc[2][4], sum[2][4];
+        auto convert = [&](int u) {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j)
+                w[u & 1][j] = weights8<BF16>(words[u % NT][u / NT * kSteps + j]);
+        };
+        auto add = [&](int u) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
             {
-#pragma unroll
-                for (int j = 0; j < kSteps; ++j)
-                    b[j][i] = as_u32x4(xs[(i * 4 + q * kSteps + j) * 64]);
-                if (BF16)
-                {
-                    sum[i] = zero;
-#pragma unroll
-                    for (int j = 0; j < kSteps; ++j)
-                        sum[i] = product<BF16>(ones, b[j][i], sum[i]);
-                }
+                f32x4& to = y[u % NT][i];
+                scaled_add<BF16>(to, acc[u & 1][i], sum[u / NT & 1][i], scale[u / NT][u % NT]);
+                asm volatile("" : "+v"(to)); // here and not behind the barrier, where every group's products would have to be kept
             }
-            // the products of output tile n are under way while n + 1 is converted and n - 1 is scaled
-            u32x4 w[2][kSteps];
-            f32x4 acc[2][4];
-            uint2 scale[2];
-            auto convert = [&](int n) {
-                const uint32_t* const words = reinterpret_cast<const uint32_t*>(ws + n * 64) + q * kSteps;
-                scale[n & 1] = *reinterpret_cast<const uint2*>(ss + q * 1024 + n * 32);
+        };
+        convert(0);
 #pragma unroll
-                for (int j = 0; j < kSteps; ++j)
-                    w[n & 1][j] = weights8<BF16>(words[j]);
-            };
-            auto add = [&](int n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    scaled_add<BF16>(y[n][i], acc[n & 1][i], sum[i], scale[n & 1]);
-            };
-            convert(0);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-            {
+        for (int u = 0; u < kUnits; ++u)
+        {
+            const int q = u / NT;
+            if (BF16 && u % NT == 0)
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        acc[n & 1][i] = product<BF16>(w[n & 1][j], b[j][i], j ? acc[n & 1][i] : zero);
-                if (n > 0)
-                    add(n - 1);
-                if (n + 1 < NT)
-                    convert(n + 1);
-            }
-            add(NT - 1);
+                        sum[q & 1][i] = product<BF16>(ones, b[q * kSteps + j][i], j ? sum[q & 1][i] : zero);
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[u & 1][i] = product<BF16>(w[u & 1][j], b[q * kSteps + j][i], j ? acc[u & 1][i] : zero);
+            if (u > 0)
+                add(u - 1);
+            if (u + 1 < kUnits)
+                convert(u + 1);
         }
+        add(kUnits - 1);
+        if (!wm)
+            arrived(t + 1);
+        meet();
     }
+    if (!wm)
+        meet();
     const bool whole = p.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -417,19 +418,20 @@ void launch_few(const tllm_group_matmul_params_t& p, hipStream_t stream)
     few_rows_kernel<BF16, GROUP, R, NT><<<grid, 64 * F::kWaves, F::kLds, stream>>>(p);
 }
 
-// The forms and what a k-tile of a workgroup takes in each (us, all CUs busy; measured over 24 to 1024 rows and 190 to 12288 outputs of fp16 with groups
-// of 128).  Every form has the CU's LDS to itself, so a product takes as many rounds as its workgroups take places, and the form with the
-// least time is the one to take: 1 x 4096 x 4096 in 256 workgroups of 16 outputs, 1024 x 11008 x 4096 in 464 tiles of 128 x 192 (121 us; 150 in tiles of
-// 256, 197 in the largest of the others), 67 x 190 x 10144 in 60 workgroups of 16 x 16 (8.5 us; 143 in tiles), 200 x 4096 x 4096 in 256 of 64 x 64
-// (20 us; 60 in tiles).
+// The forms and what a workgroup takes in each (us, all CUs busy): `once` and `each` k-tile, fitted to 256 and 1024 workgroups of fp16 with groups
+// of 128 over k of 512 to 11008, which they meet within 10 %.  A product takes as many rounds as its workgroups take CUs, and the form with the
+// least time is the one to take: 1 x 4096 x 4096 in 256 workgroups of 16 outputs, 1024 x 11008 x 4096 in 464 tiles of 128 x 192 (109 us; 126 in tiles of
+// 128, 136 in tiles of 256, 197 in tiles of 64), 1024 x 4096 x 4096 in 256 of 128 x 128 (44 us; 54 in tiles of 192), 67 x 190 x 10144 in 60 of 16 x 16 (8.5 us; 143 in
+// tiles of 192).
 struct Form
 {
     int rows, outputs;
-    float us;
+    float once, each;
 };
-constexpr Form kForms[] = {{4, 16, .07f}, {4, 32, .10f}, {4, 48, .13f}, {4, 64, .17f}, {8, 16, .07f}, {8, 32, .10f}, {8, 48, .14f}, {8, 64, .18f}, {16, 16, .09f}, {16, 32, .13f},
-    {16, 48, .17f}, {16, 64, .21f}, {32, 16, .16f}, {32, 32, .24f}, {32, 48, .29f}, {32, 64, .33f}, {64, 16, .25f}, {64, 32, .34f}, {64, 48, .50f}, {64, 64, .58f}, {128, 192, 1.88f},
-    {128, 256, 2.33f}};
+constexpr Form kForms[] = {{4, 16, 1.0f, .050f}, {4, 32, 1.3f, .077f}, {4, 48, 1.0f, .123f}, {4, 64, 1.1f, .155f}, {8, 16, 1.0f, .057f}, {8, 32, .9f, .097f}, {8, 48, 1.0f, .126f},
+    {8, 64, 1.3f, .151f}, {16, 16, .8f, .082f}, {16, 32, 1.1f, .106f}, {16, 48, 1.3f, .131f}, {16, 64, 1.6f, .165f}, {32, 16, 1.1f, .121f}, {32, 32, 1.6f, .151f},
+    {32, 48, 2.1f, .183f}, {32, 64, 2.4f, .225f}, {64, 16, 1.9f, .207f}, {64, 32, 2.5f, .229f}, {64, 48, 3.4f, .267f}, {128, 64, 2.5f, .940f}, {128, 128, 4.6f, 1.268f},
+    {128, 192, 7.2f, 1.625f}, {128, 256, 8.4f, 2.070f}};
 
 int form_of(int rows, int n, int k)
 {
@@ -440,7 +442,7 @@ int form_of(int rows, int n, int k)
     {
         const Form& f = kForms[i];
         const int64_t groups = (int64_t) ((n + f.outputs - 1) / f.outputs) * ((rows + f.rows - 1) / f.rows);
-        const double us = (double) ((groups + cus - 1) / cus) * (2. + k_tiles * (double) f.us); // 2: a round's first loads and its end
+        const double us = (double) ((groups + cus - 1) / cus) * ((double) f.once + k_tiles * (double) f.each);
         if (us < least)
         {
             least = us;
@@ -459,7 +461,7 @@ void launch_form(const tllm_group_matmul_params_t& p, hipStream_t stream)
         f.outputs == 16 ? launch_few<BF16, GROUP, R, 1>(p, stream)                                                     \
             : f.outputs == 32 ? launch_few<BF16, GROUP, R, 2>(p, stream)                                               \
             : f.outputs == 48 ? launch_few<BF16, GROUP, R, 3>(p, stream)                                               \
-                              : launch_few<BF16, GROUP, R, 4>(p, stream);                                              \
+                              : launch_few<BF16, GROUP, R, (R < 16 ? 4 : 3)>(p, stream);                               \
         break;
     switch (f.rows)
     {
@@ -468,7 +470,11 @@ void launch_form(const tllm_group_matmul_params_t& p, hipStream_t stream)
         TLLM_FEW(4)
         TLLM_FEW(8)
         TLLM_FEW(16)
-    default: f.outputs == 192 ? launch_tiles<BF16, GROUP, 3>(p, stream) : launch_tiles<BF16, GROUP, 4>(p, stream);
+    default:
+        f.outputs == 64 ? launch_tiles<BF16, GROUP, 1>(p, stream)
+            : f.outputs == 128 ? launch_tiles<BF16, GROUP, 2>(p, stream)
+            : f.outputs == 192 ? launch_tiles<BF16, GROUP, 3>(p, stream)
+                               : launch_tiles<BF16, GROUP, 4>(p, stream);
     }
 #undef TLLM_FEW
 }
