@@ -101,7 +101,9 @@ __device__ __forceinline__ void dma16(const void* from, uint32_t lds_byte)
 
 // 4 R rows x 16 NT outputs a workgroup; its waves share the k-tiles out and join through LDS.  What it has to read is the weights, once;
 // each CU also reads all of x, which is as much as its weights at 8 rows and 16 outputs and is why x comes by whole 256-byte pieces of the
-// rows that there are.  A wave has a ring of DEEP k-tiles in LDS, its own: no barrier, only the count of what is under way.
+// rows that there are.  A wave has a ring of kDeep k-tiles in LDS, its own: no barrier, only the count of what is under way; where LDS holds
+// one k-tile a wave, 8 waves with one hide more than 4 with two (64 x 12288 x 4096: 16.3 us, 20.6).  Bound by the weights' bytes and, from 16 rows on, by x
+// on its way from L2 (1 x 4096 x 4096 4.7 us, of them 2 the launch and the join; 8 x 4096 x 11008 in bfloat16 8.0; 24 x 12288 x 4096 10.6).
 template <int R, int NT>
 struct FewForm
 {
@@ -225,8 +227,13 @@ __global__ __launch_bounds__((64 * FewForm<R, NT>::kWaves)) void few_rows_kernel
 }
 
 // Many rows: 128 rows x 64 NT outputs a workgroup of 8 waves, 64 x 16 NT a wave.  x, weights and scales of a k-tile go to LDS by DMA, x and weights as the
-// fragments that the waves read back (64 lanes x 16 bytes in a row: no conflicts), three k-tiles in a ring: two are under way while one is
-// multiplied.  One barrier a k-tile: behind it the tile before is free and the next but one is sent for.
+// fragments that the waves read back (64 lanes x 16 bytes in a row: no conflicts), three k-tiles in a ring.
+// The two waves of a SIMD are half a k-tile apart: while the one multiplies, converts and scales, the other reads its fragments (in step with each
+// other all waves wait for LDS, then all convert, then all multiply: 1024 x 11008 x 4096 122 us, 110 so).  Two barriers a k-tile keep them there, one more at
+// the start for the later half and one at the end for the earlier.  Between barriers 2 t - 1 and 2 t the earlier half reads k-tile t, which every
+// wave has waited for before barrier 2 t - 1; the later half reads it between 2 t and 2 t + 1; whoever sends for k-tile t + 2 has passed barrier 2 t - 1,
+// before which both have read t - 1, whose place it takes.
+// 0.84 PFLOP/s; with the matrix instructions alone 1.2, what power leaves of them (a library product of 8192^3: 1.3).
 constexpr int kStages = 3;
 
 template <int GROUP, int NT>
