@@ -1,5 +1,8 @@
 """The operators of a quantised serving step (include/tllm_serving_api.h) through their Python entry points, against oracle/serving_oracle.py: page
 plans and the cache's bits exactly, attention and 4-bit products within bounds that follow from their arithmetic (next to each assert)."""
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -484,6 +487,13 @@ def test_group_matmul_in_every_form(rows, n, group, dtype):
     check_product(np.random.default_rng(n), rows, n, 288, group, dtype)
 
 
+@pytest.mark.parametrize('group,dtype', [(128, 'fp16'), (32, 'bf16'), (64, 'fp16')])
+@pytest.mark.parametrize('k', [32, 128, 160, 256, 384, 512])
+@pytest.mark.parametrize('rows,n', [(1500, 1100), (400, 1530), (2300, 2500)])
+def test_group_matmul_of_few_k_tiles(rows, n, k, group, dtype):
+    check_product(np.random.default_rng(rows + k), rows, n, k, group, dtype)
+
+
 @pytest.mark.parametrize('rows', [1, 9, 40, 300])
 @pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
 def test_group_matmul_strided(rows, dtype):
@@ -642,6 +652,26 @@ def test_attention_in_place_of_its_queries(spans, dtype):
     want = cache.attention(q, *args)
     assert cache.attention(q, *args, out=q) is q
     assert torch.equal(q, want) and torch.equal(qkv[:, 6:], kept[:, 6:])
+
+
+def test_copies_have_tensors_of_their_own():
+    torch.manual_seed(3)
+    mm, cache = G.GroupQuantMatmul.from_float(torch.randn((50, 96), device='cuda'), 32), P.PagedKV8Cache.empty(2, 16, 1, 64)
+    x, kv, q = torch.randn((3, 96), device='cuda').half(), torch.randn((5, 2, 64), device='cuda').half(), torch.randn((5, 2, 64), device='cuda').half()
+    table, cu, lens = gpu([[1]]), gpu([0, 5]), gpu([5])
+    cache.append(kv[:, :1], kv[:, 1:], gpu(range(16, 21)))
+    want, seen = mm(x), cache.attention(q, table, cu, lens, 5)
+    for make in (copy.copy, copy.deepcopy, lambda thing: pickle.loads(pickle.dumps(thing))):
+        mm2, cache2 = make(mm), make(cache)
+        if make is not copy.copy:
+            assert mm2.packed.data_ptr() != mm.packed.data_ptr() and cache2.pool.data_ptr() != cache.pool.data_ptr()
+            kept = [t.clone() for t in (mm.packed, mm.scales, cache.pool, cache.scales)]
+            for t in (mm.packed, mm.scales, cache.pool, cache.scales):
+                t.zero_()
+        assert torch.equal(mm2(x), want) and torch.equal(cache2.attention(q, table, cu, lens, 5), seen)
+        if make is not copy.copy:
+            for t, was in zip((mm.packed, mm.scales, cache.pool, cache.scales), kept):
+                t.copy_(was)
 
 
 def test_tensors_of_the_objects_stay():

@@ -1,5 +1,6 @@
 """include/tllm_serving_api.h without a GPU: the entry points are exported, and refuse on the host, with a reason, what their kernels do not take; the
 weights' packing is the documented layout; the oracle's own pieces agree with each other."""
+import copy
 import ctypes
 import os
 import re
@@ -220,6 +221,11 @@ def test_caches_and_pools_refuse():
     b = P.DeviceBlockPool(4, 16, 2, 3, device='cpu')
     with pytest.raises(ValueError, match='GPU'):
         b.plan(torch.tensor([1, 1], dtype=torch.int32), 2)
+    for other in (dict(), dict(lens=b.lens), dict(ring_state=b.ring_state)):  # it would leave the pool's own state behind
+        with pytest.raises(ValueError, match='over this pool'):
+            b.plan(torch.tensor([1, 1], dtype=torch.int32), 2, P.StepPlan(2, 2, 'cpu', **other))
+    with pytest.raises(TypeError, match='copied'):
+        copy.copy(P.StepPlan(2, 2, 'cpu'))
 
 
 def test_the_oracle_keeps_what_it_is_given():

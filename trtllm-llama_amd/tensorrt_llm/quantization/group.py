@@ -1,6 +1,7 @@
 """Linear layers with 4-bit weights and a scale for each group of a row (ctypes binding of tllm_group_matmul, include/tllm_serving_api.h).
 
-Next to WeightOnlyQuantMatmul, whose 4-bit weights have one scale for a whole output channel.  y = x W^T, W[n, k] = q[n, k] s[n, k / group]."""
+Next to WeightOnlyQuantMatmul, whose 4-bit weights have one scale for a whole output channel.  y = x W^T, W[n, k] = q[n, k] s[n, k / group].  There are no
+gradients: the product serves."""
 import ctypes
 import struct
 from typing import Optional, Tuple
@@ -72,15 +73,26 @@ def pack(q: torch.Tensor, scales: torch.Tensor, group: int) -> Tuple[torch.Tenso
     return u.reshape(tiles, steps, 64, 16).contiguous(), s
 
 
+def _restored(cls, *held):
+    layer = cls.__new__(cls)
+    layer._hold(*held)
+    return layer
+
+
 class GroupQuantMatmul(Fixed):
     """y = x W^T with W packed once: q int8 [n, k] in -8 .. 7, scales float16 or bfloat16 [n, ceil(k / group)], which is the type of x and y too."""
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, group: int):
-        self.n, self.k, self.group, self.dtype = q.shape[0], q.shape[1], group, scales.dtype
-        self.packed, self.scales = pack(q, scales, group)
+        self._hold(*q.shape, group, *pack(q, scales, group))
+
+    def _hold(self, n, k, group, packed, scales):
+        self.n, self.k, self.group, self.dtype, self.packed, self.scales = n, k, group, scales.dtype, packed, scales
         if self.packed.device.type != 'cuda':
             raise ValueError(f'the weights have to be on a GPU: got {self.packed.device}')
         self._index, self._act, self._at = self.packed.get_device(), _ACT[self.dtype], (self.packed.data_ptr(), self.scales.data_ptr())
+
+    def __reduce_ex__(self, protocol):  # copies have addresses of their own
+        return _restored, (type(self), self.n, self.k, self.group, self.packed, self.scales)
 
     @classmethod
     def from_float(cls, weight: torch.Tensor, group: int, dtype=torch.float16) -> 'GroupQuantMatmul':

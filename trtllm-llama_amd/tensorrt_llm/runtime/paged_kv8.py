@@ -4,7 +4,8 @@ Where KVCacheManager hands out block ids on the host, `DeviceBlockPool` keeps th
 `plan` a step serves every layer, and nothing of it comes back to the host, so a step with it can be captured into a graph.  `PagedKV8Cache` is one
 layer's cache: int8 or e4m3 elements (torch.int8, torch.float8_e4m3fn) under a scale for each page and head, filled by `append` and read by
 `attention`.  Tensors are handed over as device pointers; calls run on torch's current stream of the tensors' device and check their
-arguments (TypeError, ValueError; RuntimeError with the library's reason).  A failing call has launched nothing."""
+arguments (TypeError, ValueError; RuntimeError with the library's reason).  A failing call has launched nothing.  There are no gradients: these
+operators serve."""
 import ctypes
 import struct
 from typing import Optional
@@ -111,6 +112,9 @@ class StepPlan(Fixed):
         self.n_seqs, self.n_rows, self.index, self.cu_tokens, self.slot_map, self.positions, self.status, self.lens, self.ring_state, self._at = (
             n_seqs, n_rows, index, cu, slots, places, status, lens, ring_state, at)
 
+    def __reduce_ex__(self, protocol):
+        raise TypeError('a StepPlan is not copied: make another one')
+
 
 def plan_step(lens: torch.Tensor, new_lens: torch.Tensor, ring: torch.Tensor, ring_state: torch.Tensor, block_table: torch.Tensor, page_size: int,
               n_rows: int, out: Optional[StepPlan] = None) -> StepPlan:
@@ -153,6 +157,8 @@ class DeviceBlockPool(object):
         nothing and says why in out.status; as it has no rows, what the step launches behind it touches nothing."""
         if out is None:
             out = StepPlan(self.max_seqs, n_rows, self.lens.device, lens=self.lens, ring_state=self.ring_state)
+        elif out.lens.data_ptr() != self.lens.data_ptr() or out.ring_state.data_ptr() != self.ring_state.data_ptr():
+            raise ValueError('out has to be a plan over this pool: StepPlan(.., lens=pool.lens, ring_state=pool.ring_state)')
         return plan_step(self.lens, new_lens, self.ring, self.ring_state, self.block_table, self.page_size, n_rows, out)
 
 
@@ -180,6 +186,9 @@ class PagedKV8Cache(Fixed):
         self.pool, self.scales, self.page_size, self.head_size = pool, scales, page_size, head_size
         self.blocks, self.kv_heads, self._type = pool.shape[0], pool.shape[2], _CACHE[pool.dtype]
         self._index, self._at = pool.get_device(), (pool.data_ptr(), scales.data_ptr())
+
+    def __reduce_ex__(self, protocol):  # copies have addresses of their own
+        return type(self), (self.pool, self.scales, self.page_size, self.head_size)
 
     @classmethod
     def empty(cls, blocks: int, page_size: int, kv_heads: int, head_size: int, dtype=torch.int8, device='cuda') -> 'PagedKV8Cache':
