@@ -17,9 +17,9 @@
 //               whose parts merge_kernel joins (131072 keys of one request: 42 + 4 us; a token over 1032, 32 heads: 7 + 4, the chain table -> keys ->
 //               softmax -> join).
 //   tile_kernel 64 or 128 rows: the waves share the tiles, which they bring to LDS as fp16 fragments, the next one while this one is computed.  Prompts
-//               are bound by the arithmetic - products, exponentials, and the conversions, which are once a workgroup here and not once a wave: 0.87
-//               PFLOP/s where workgroups fill the chip evenly (2048 tokens behind 20000, 32 heads of 128), 0.58 where 640 of them have 512 places (three
-//               prompts of up to 1024 behind up to 2500: 197 us).
+//               are bound by the arithmetic - products, exponentials, and the conversions, which are once a workgroup here and not once a wave: 0.90
+//               PFLOP/s where workgroups fill the chip evenly (2048 tokens behind 20000, 32 heads of 128), 0.62 where 640 of them have 512 places (three
+//               prompts of up to 1024 behind up to 2500: 184 us).
 #include "dev_utils.h"
 #include "launch_util.h"
 #include "serving_kernels.h"
@@ -472,7 +472,7 @@ struct TileForm
     static constexpr int kKeyFrags = 4 * DIM / 32, kFrags = 2 * kKeyFrags; // of 1 KB: keys [part][k-step], values [channels / 16][k-step]
     static constexpr int kAhead = DIM == 256 ? 2 : 4; // fragments that are read ahead of their products
     // Tiles that LDS holds: two, one computed and one arriving; of heads of 256 one, so that two workgroups fit a CU (with some 30 registers a lane
-    // spilled; 1024 tokens behind 1500, 32 heads: 116 us, one workgroup 183)
+    // spilled; 1024 tokens behind 1500, 32 heads: 105 us, one workgroup a half more)
     static constexpr int kBuffers = DIM == 256 ? 1 : 2, kLds = kBuffers * kFrags * 1024;
 };
 
@@ -485,12 +485,16 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
     using F = TileForm<DIM>;
     constexpr int kSteps = DIM / 32, kOut = DIM / 16, RT = F::kRt;
     extern __shared__ u32x4 frags[]; // [kBuffers][kFrags][64]
-    // Workgroups go round the XCDs: the row tiles of one request and head follow each other on one XCD, whose L2 holds their keys.  Those with the
-    // most keys first, and the other way round where a pair of request and head begins in an odd 32: workgroups 32 apart of an XCD meet on
-    // one CU (2048 tokens behind 1500, 32 heads of 128: 125 us, 148 without)
-    const int id = blockIdx.x - light_groups, xcd = id & 7, at8 = id >> 3, order = at8 % row_tiles;
-    const int tile = id < 0 ? 0 : (at8 - order) >> 5 & 1 ? order : row_tiles - 1 - order;
-    const int part = id < 0 ? blockIdx.x % light.parts : blockIdx.y, pair = id < 0 ? blockIdx.x / light.parts : at8 / row_tiles * 8 + xcd;
+    // Workgroups go round the XCDs.  Those of an XCD take the row tiles of as many pairs of request and key head as fill its places, then the next
+    // ones': the tiles of a pair walk its keys side by side, which the XCD's L2 holds, and the tiles with the most keys begin first, so that
+    // the last ones to begin are short (12 requests of up to 700, 32 heads of 128: 117 us, 125 pair after pair; 4 of 1024 behind 3000, 32 heads on 8: 223, 234).  Where
+    // every tile has a place from the start, the second half comes the other way round: workgroups 32 apart of an XCD meet on one CU, a light one
+    // beside a heavy one (2048 tokens behind 1500, 32 heads of 128: 114 us, 116 without, 126 pair after pair; heads of 64: 79, 82, 91).
+    const int id = blockIdx.x - light_groups, xcd = id & 7, pairs8 = (p.n_seqs * p.kv_heads + 7) >> 3, mine = pairs8 * row_tiles;
+    const int at8 = mine <= 64 && id >> 3 >= 32 ? 32 + mine - 1 - (id >> 3) : id >> 3;
+    const int most = max(1, 64 / row_tiles), turn = at8 / (most * row_tiles), in = at8 - turn * (most * row_tiles), width = min(most, pairs8 - turn * most);
+    const int tile = id < 0 ? 0 : row_tiles - 1 - in / width;
+    const int part = id < 0 ? blockIdx.x % light.parts : blockIdx.y, pair = id < 0 ? blockIdx.x / light.parts : (turn * most + in % width) * 8 + xcd;
     if (pair >= p.n_seqs * p.kv_heads)
         return;
     const int head = pair % p.kv_heads, b = pair / p.kv_heads, group = p.q_heads / p.kv_heads;
