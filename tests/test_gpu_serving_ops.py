@@ -373,6 +373,13 @@ def test_attention_split_over_workgroups(spans, max_kv, kind, dtype, size):
     check_attention(np.random.default_rng(size), kind, dtype, 64, size, 1, 3, spans, max_kv=max_kv, spare_rows=1)
 
 
+@pytest.mark.parametrize('kind,dtype,size', [('int8', 'fp16', 128), ('fp8', 'bf16', 64), ('int8', 'bf16', 64), ('fp8', 'fp16', 128), ('int8', 'fp16', 256)])
+@pytest.mark.parametrize('spans,max_kv,window', [([(500, 1)], None, 0), ([(290, 1), (0, 0), (511, 1), (64, 2)], None, 0), ([(900, 1), (1, 1)], None, 0), ([(3000, 1), (10, 1)], 400, 0),
+                                                 ([(3000, 3), (449, 1)], None, 300)])
+def test_attention_of_few_keys(spans, max_kv, window, kind, dtype, size):
+    check_attention(np.random.default_rng(size), kind, dtype, 64, size, 2, 3, spans, max_kv=max_kv, window=window, spare_rows=1)
+
+
 @pytest.mark.parametrize('size', [64, 256])
 def test_attention_of_many_workgroups(size):
     """More than 32 row tiles an XCD, in numbers that do not divide it: every row is computed, and once."""

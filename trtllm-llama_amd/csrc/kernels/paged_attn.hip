@@ -12,7 +12,7 @@
 // softmax scale behind the first product; the value's, relative to the largest value scale so far and times 2^7, in the exponent of the
 // weight.  m is brought along only when a score is more than 8 (a factor of 2^8) above it: a weight is at most 2^15, nothing overflows, it keeps
 // its 11 bits until its page's scale is 2^-21 of another's, and in most tiles no lane asks another for anything.
-//   rows_body   16 rows: four waves take tiles in turn, straight from memory into registers, and join through LDS.  Single tokens are bound by the
+//   rows_body   16 rows: four or eight waves take tiles in turn, straight from memory into registers, and join through LDS.  Single tokens are bound by the
 //               cache's bytes (48 requests over 4000 to 8000 keys, 8 key heads of 128, e4m3: 111 us, 5.4 TB/s); the keys are also split over workgroups,
 //               whose parts merge_kernel joins (131072 keys of one request: 42 + 4 us; a token over 1032, 32 heads: 7 + 4, the chain table -> keys ->
 //               softmax -> join).
@@ -41,7 +41,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kPShift = 7.f, kSlack = 8.f; // see above
-constexpr int kTile = 64, kRowWaves = 4; // keys; waves of rows_body
+constexpr int kTile = 64;
 
 __device__ __forceinline__ f16x8 join(u32x4 w)
 {
@@ -252,22 +252,22 @@ __device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], float& m, 
     w[1] = join(p[1]);
 }
 
-template <int DIM>
+template <int DIM, int NW>
 struct RowsLds
 {
     static constexpr int kLine = DIM + 4;
-    static constexpr int kBytes = (kRowWaves / 2 * 16 * kLine + kRowWaves * 32) * 4;
+    static constexpr int kBytes = (NW / 2 * 16 * kLine + NW * 32) * 4;
 };
 
 // 16 rows (`tile`) of a request and key head, keys of one part
-template <int DIM, bool BF16, bool FP8>
+template <int DIM, bool BF16, bool FP8, int NW>
 __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p, const int shift, const Split& split, const Request& req, int head, int b, int tile, int part,
     float* lds)
 {
-    constexpr int kSteps = DIM / 32, kOut = DIM / 16, kLine = RowsLds<DIM>::kLine, kPlaces = kRowWaves / 2;
+    constexpr int kSteps = DIM / 32, kOut = DIM / 16, kLine = RowsLds<DIM, NW>::kLine, kPlaces = NW / 2;
     float(*acc)[16][kLine] = reinterpret_cast<float(*)[16][kLine]>(lds);
     float(*ms)[16] = reinterpret_cast<float(*)[16]>(lds + kPlaces * 16 * kLine);
-    float(*ls)[16] = ms + kRowWaves;
+    float(*ls)[16] = ms + NW;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
     const int group = p.q_heads / p.kv_heads;
     const int rows = min(req.rows, p.max_new) * group, row = tile * 16 + r;
@@ -322,8 +322,8 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
         vb_now = vb;
         fetch_keys(t0);
         fetch_values(t0, vb_now);
-        if (t0 + kRowWaves < t_end)
-            blocks_of(t0 + kRowWaves);
+        if (t0 + NW < t_end)
+            blocks_of(t0 + NW);
     }
     f16x8 q[kSteps];
     const uint16_t* const q_row = live ? static_cast<const uint16_t*>(p.q) + (req.row0 + token) * p.q_row + qh * p.q_head : nullptr;
@@ -359,9 +359,9 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
         const int vb_next = vb;
         if constexpr (more)
         {
-            fetch_keys(t + kRowWaves);
-            if (t + 2 * kRowWaves < t_end)
-                blocks_of(t + 2 * kRowWaves);
+            fetch_keys(t + NW);
+            if (t + 2 * NW < t_end)
+                blocks_of(t + 2 * NW);
         }
         const TileScales scales = scales_of(ks, vs, ref);
         const int keep = v_in ? req.len - vk : 0;
@@ -379,12 +379,12 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
         }
         vb_now = vb_next;
         if constexpr (more)
-            fetch_values(t + kRowWaves, vb_now);
+            fetch_values(t + NW, vb_now);
     };
     if (t0 < t_end)
     {
         int t = t0;
-        for (; t + kRowWaves < t_end; t += kRowWaves)
+        for (; t + NW < t_end; t += NW)
             step(t, std::true_type{});
         step(t, std::false_type{});
     }
@@ -399,7 +399,7 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
     __syncthreads();
     float m_all = ms[0][r];
 #pragma unroll
-    for (int w = 1; w < kRowWaves; ++w)
+    for (int w = 1; w < NW; ++w)
         m_all = fmaxf(m_all, ms[w][r]);
     const float mine = __builtin_amdgcn_exp2f(m - (m_all == -INFINITY ? 0.f : m_all)) * (ref.v * __builtin_amdgcn_exp2f(-kPShift));
     if (wave >= kPlaces)
@@ -415,19 +415,19 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
             *at = *at + o[i] * mine;
         }
     __syncthreads();
-    for (int u = tid; u < 16 * DIM / 4; u += 64 * kRowWaves)
+    for (int u = tid; u < 16 * DIM / 4; u += 64 * NW)
     {
         const int ur = u / (DIM / 4), d = u % (DIM / 4) * 4, urow = tile * 16 + ur;
         if (urow >= rows)
             continue;
         float um = ms[0][ur];
 #pragma unroll
-        for (int w = 1; w < kRowWaves; ++w)
+        for (int w = 1; w < NW; ++w)
             um = fmaxf(um, ms[w][ur]);
         const float uu = um == -INFINITY ? 0.f : um;
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kRowWaves; ++w)
+        for (int w = 0; w < NW; ++w)
             sum += ls[w][ur] * __builtin_amdgcn_exp2f(ms[w][ur] - uu);
         f32x4 a = *reinterpret_cast<const f32x4*>(&acc[0][ur][d]);
 #pragma unroll
@@ -452,17 +452,17 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
 }
 
 // a workgroup per request, key head and part of the keys: rows of one tile
-template <int DIM, bool BF16, bool FP8>
-__global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const tllm_paged_attention_params_t p, const int shift, const Split split)
+template <int DIM, bool BF16, bool FP8, int NW>
+__global__ __launch_bounds__(64 * NW) void rows_kernel(const tllm_paged_attention_params_t p, const int shift, const Split split)
 {
-    __shared__ f32x4 lds[RowsLds<DIM>::kBytes / 16];
+    __shared__ f32x4 lds[RowsLds<DIM, NW>::kBytes / 16];
     int id = blockIdx.x;
     const int part = id % split.parts;
     id /= split.parts;
     const int head = id % p.kv_heads, b = id / p.kv_heads;
     const Request req = request_of(p, b, shift);
     if (req.rows > 0)
-        rows_body<DIM, BF16, FP8>(p, shift, split, req, head, b, 0, part, reinterpret_cast<float*>(lds));
+        rows_body<DIM, BF16, FP8, NW>(p, shift, split, req, head, b, 0, part, reinterpret_cast<float*>(lds));
 }
 
 template <int DIM>
@@ -505,7 +505,7 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
     if (rows <= 16)
     {
         if (blockIdx.y == 0 && (id < 0 || light_groups == 0))
-            rows_body<DIM, BF16, FP8>(p, shift, light, req, head, b, 0, part, reinterpret_cast<float*>(frags));
+            rows_body<DIM, BF16, FP8, 4>(p, shift, light, req, head, b, 0, part, reinterpret_cast<float*>(frags));
         return;
     }
     if (id < 0)
@@ -801,6 +801,7 @@ int row_tiles_of(const tllm_paged_attention_params_t& p) // of tile_kernel
 // More rows: what fills two places on every CU, where their tiles do not (443 tokens of one head over 57000 keys: 7 tiles).
 struct Parts
 {
+    int waves; // of rows_kernel
     int light, heavy, per; // of requests of one tile of rows, of the others; rows that one of the light ones has at most
 };
 Parts parts_of(const tllm_paged_attention_params_t& p)
@@ -808,7 +809,7 @@ Parts parts_of(const tllm_paged_attention_params_t& p)
     const int64_t pairs = (int64_t) p.n_seqs * p.kv_heads, cus = launch_util::device_cus();
     const int64_t keys = p.window > 0 ? std::min<int64_t>((int64_t) p.window + p.max_new, p.max_kv) : p.max_kv;
     auto within = [](int64_t want, int64_t most) { return (int) std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64)); };
-    Parts s = {1, 1, std::min(p.max_new, 16 / (p.q_heads / p.kv_heads))};
+    Parts s = {4, 1, 1, std::min(p.max_new, 16 / (p.q_heads / p.kv_heads))};
     int64_t few = pairs, least = pairs >= cus ? 2048 : pairs * 4 >= cus ? 512 : 128;
     if (!one_tile(p))
     {
@@ -818,6 +819,13 @@ Parts parts_of(const tllm_paged_attention_params_t& p)
     }
     if (few > 0)
         s.light = within(((few < cus ? 2 : 4) * cus + few - 1) / few, keys / least);
+    // Few keys are not split: eight waves of one workgroup and no second launch (500 keys, 32 heads of 128: 9.1 us, 10.0 in parts, 1032: 13.2 and 11.0;
+    // 1032 keys, 4 x 8 heads of 64: 8.4 and 9.0, 2048: 11.5 and 10.1).  Heads of 256 have no registers for eight.
+    if (one_tile(p) && s.light > 1 && keys * p.head_size <= 65536 && p.head_size < 256)
+    {
+        s.light = 1;
+        s.waves = 8;
+    }
     return s;
 }
 
@@ -841,7 +849,15 @@ void launch_form(const tllm_paged_attention_params_t& p, void* workspace, hipStr
     float* const ml = o + (n.light + n.heavy) * DIM;
     const Split light = {o, ml, s.light, s.per}, heavy = {o + n.light * DIM, ml + n.light * 2, s.heavy, 0};
     if (one_tile(p))
-        rows_kernel<DIM, BF16, FP8><<<(unsigned) (pairs * s.light), 256, 0, stream>>>(p, shift, light);
+    {
+        if constexpr (DIM < 256)
+            if (s.waves == 8)
+            {
+                rows_kernel<DIM, BF16, FP8, 8><<<(unsigned) (pairs * s.light), 512, 0, stream>>>(p, shift, light);
+                return;
+            }
+        rows_kernel<DIM, BF16, FP8, 4><<<(unsigned) (pairs * s.light), 256, 0, stream>>>(p, shift, light);
+    }
     else
     {
         using F = TileForm<DIM>;
