@@ -56,7 +56,7 @@ def check_plan(lens, new, ring, state, table, page, n_rows, in_place=False, pad=
 
 
 @pytest.mark.parametrize('in_place', [False, True])
-@pytest.mark.parametrize('n,page,longest,most', [(1, 64, 0, 1), (1, 16, 100, 1000), (7, 32, 90, 40), (64, 64, 700, 1), (300, 16, 60, 30), (4096, 128, 300, 2), (33, 64, 64, 3000)])
+@pytest.mark.parametrize('n,page,longest,most', [(1, 64, 0, 1), (1, 16, 100, 1000), (7, 32, 90, 40), (64, 64, 700, 1), (300, 16, 60, 30), (4096, 128, 300, 2), (33, 64, 64, 3000), (4096, 128, 300, 127)])
 def test_plan(n, page, longest, most, in_place):
     rng = np.random.default_rng(n * 131 + page)
     wide = -(-(longest + most) // page) + 1
@@ -187,7 +187,7 @@ def test_append_to_the_bit(page, size, heads, spans, dtype, kind):
     c.same()
 
 
-@pytest.mark.parametrize('spans', [[(5, 1100)], [(i, 1) for i in range(300)] + [(0, 900)], [(100, 3000), (0, 1), (31, 1), (63, 2), (0, 1300)]], ids=['one', 'tokens', 'prompts'])
+@pytest.mark.parametrize('spans', [[(5, 1100)], [(i, 1) for i in range(300)] + [(0, 900)], [(100, 3000), (0, 1), (31, 1), (63, 2), (0, 1300)], [(40, 70000)]], ids=['one', 'tokens', 'prompts', 'most'])
 def test_append_of_many_rows(spans):
     """Workgroups that look for runs in 16 rows, and in a page of rows."""
     rng = np.random.default_rng(len(spans))
@@ -482,7 +482,7 @@ def check_product(rng, rows, n, k, group, dtype, strided=False):
 @pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
 @pytest.mark.parametrize('group', [32, 64, 128])
 @pytest.mark.parametrize('rows,n,k', [(1, 16, 32), (1, 1, 128), (1, 4096, 4096), (3, 100, 160), (16, 257, 992), (17, 64, 1024), (32, 130, 96), (33, 513, 2080), (64, 96, 11008),
-                                      (65, 200, 256), (130, 300, 640), (257, 1000, 1312), (700, 31, 224), (1, 4097, 4128), (5, 2050, 1056)])
+                                      (65, 200, 256), (130, 300, 640), (257, 1000, 1312), (700, 31, 224), (1, 4097, 4128), (5, 2050, 1056), (1 << 19, 5, 32)])
 def test_group_matmul(rows, n, k, group, dtype):
     check_product(np.random.default_rng(rows + n + k), rows, n, k, group, dtype)
 

@@ -817,7 +817,7 @@ Parts parts_of(const tllm_paged_attention_params_t& p)
         few = s.per ? std::min<int64_t>(p.n_seqs - 1, ((int64_t) p.n_seqs * p.max_new - p.n_rows) / (p.max_new - s.per)) * p.kv_heads : 0;
         least = 1024;
     }
-    if (few > 0)
+    if (few > 0 && (int64_t) p.n_seqs * s.per * p.q_heads <= 1 << 23) // what merge_kernel's launch takes
         s.light = within(((few < cus ? 2 : 4) * cus + few - 1) / few, keys / least);
     // Few keys are not split: eight waves of one workgroup and no second launch (500 keys, 32 heads of 128: 9.1 us, 10.0 in parts, 1032: 13.2 and 11.0;
     // 1032 keys, 4 x 8 heads of 64: 8.4 and 9.0, 2048: 11.5 and 10.1).  Heads of 256 have no registers for eight.
