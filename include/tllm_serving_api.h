@@ -131,6 +131,7 @@ int32_t tllm_paged_attention(const tllm_paged_attention_params_t* p, void* works
 /* ------------------------------------------------------------------------------------------------
  * y[m, n] = sum_k x[m, k] q[n, k] s[n, k / group], q in -8 .. 7, group 32, 64 or 128, K a multiple of 32 (the last group may be
  * shorter).  x, y and s fp16 or bfloat16 (one type), sums in fp32.
+ * bfloat16 rows hold values below 2^113; a row with larger ones or infinities gives NaN (in fp16 an infinity gives what q x gives: an infinity, or NaN for q = 0).
  * The weights are packed once (tensorrt_llm.quantization.group does it):
  *   packed  [ceil(N / 16)][ceil(K / 128)][64][16] bytes: lane l = 16 g + r of a tile holds, in its 32-bit word j, row r's eight
  *           elements k = 32 j + 8 g + e of the tile, as nibbles q + 8 in the order e = 0 2 4 6 1 3 5 7; padding is 8 (zero);

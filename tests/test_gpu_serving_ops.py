@@ -416,6 +416,28 @@ def test_attention_passes_over_entries_that_are_no_blocks():
         check_attention(rng, 'fp8', 'fp16', 32, 64, 2, 2, spans, bad=bad)
 
 
+@pytest.mark.parametrize('size', [64, 128, 256])
+@pytest.mark.parametrize('spans', [[(9, 3), (300, 2)], [(400, 2), (5000, 1)], [(100, 90), (700, 200), (40, 1)]], ids=['few', 'split', 'prompts'])
+def test_attention_keeps_what_is_not_finite_to_its_row(spans, size):
+    torch.manual_seed(size)
+    pages = [-(-length // 64) for length, _ in spans]
+    cache = P.PagedKV8Cache(torch.randint(-127, 128, (sum(pages), 2, 2, 64 * size), dtype=torch.int8, device='cuda'), torch.full((sum(pages), 2, 2), 1 / 127, device='cuda'), 64, size)
+    table, ids = torch.zeros((len(spans), max(pages)), dtype=torch.int32, device='cuda'), torch.randperm(sum(pages), dtype=torch.int32, device='cuda')
+    for b, n in enumerate(pages):
+        table[b, :n] = ids[sum(pages[:b]):sum(pages[:b + 1])]
+    rows = [new for _, new in spans]
+    args = table, gpu(np.cumsum([0] + rows)), gpu([length for length, _ in spans]), max(rows)
+    q = torch.randn((sum(rows), 4, size), device='cuda').half()
+    clean, bad = cache.attention(q, *args), q.clone()
+    bad[1, 2, 5], bad[-1, 0, 0] = float('nan'), float('nan')
+    got = cache.attention(bad, *args)
+    odd = torch.zeros(q.shape[:2], dtype=torch.bool, device='cuda')
+    odd[1, 2] = odd[-1, 0] = True
+    assert got[odd].isnan().all()
+    # values are at most 1: each of the two is off by the weights' rounding, 2^-11, sums, 2^-19, and its own, 2^-11
+    assert ((got[~odd].float() - clean[~odd].float()).abs() <= 2 * (2.0**-10 + 2.0**-19)).all()
+
+
 @pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
 def test_attention_of_far_scales(dtype):
     """Pages whose value scales are far from each other, and scores far beyond exp's range on both sides."""
@@ -499,6 +521,24 @@ def test_group_matmul_in_every_form(rows, n, group, dtype):
 @pytest.mark.parametrize('rows,n', [(1500, 1100), (400, 1530), (2300, 2500)])
 def test_group_matmul_of_few_k_tiles(rows, n, k, group, dtype):
     check_product(np.random.default_rng(rows + k), rows, n, k, group, dtype)
+
+
+@pytest.mark.parametrize('rows,n', [(3, 40), (40, 100), (200, 300), (1500, 1100)])
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+def test_group_matmul_keeps_what_is_not_finite_to_its_row(rows, n, dtype):
+    rng = np.random.default_rng(rows)
+    q = torch.from_numpy(rng.integers(1, 8, (n, 160)).astype(np.int8)).cuda()
+    f = G.GroupQuantMatmul(q, torch.from_numpy(rng.uniform(0.01, 0.2, (n, 3))).to(TYPES[dtype]).cuda(), 64)
+    x = torch.from_numpy(rng.standard_normal((rows, 160)).astype(np.float32)).to(TYPES[dtype]).cuda()
+    clean = f(x)
+    bad = x.clone()
+    bad[1, 33], bad[rows // 2, 150], bad[rows - 1, 0] = float('inf'), float('nan'), float('-inf')
+    got, odd = f(bad), sorted({1, rows // 2, rows - 1})
+    assert not got[odd].float().isfinite().any()
+    if dtype == 'fp16' and rows > 3:
+        assert (got[1] == float('inf')).all() and (got[rows - 1] == float('-inf')).all()
+    same = [i for i in range(rows) if i not in odd]
+    assert torch.equal(got[same], clean[same])
 
 
 @pytest.mark.parametrize('rows', [1, 9, 40, 300])

@@ -428,7 +428,7 @@ void launch_few(const tllm_group_matmul_params_t& p, hipStream_t stream)
 // The forms and what a workgroup takes in each (us, all CUs busy): `once` and `each` k-tile, fitted to 256 and 1024 workgroups of fp16 with groups
 // of 128 over k of 512 to 11008, which they meet within 10 %.  A product takes as many rounds as its workgroups take CUs, and the form with the
 // least time is the one to take: 1 x 4096 x 4096 in 256 workgroups of 16 outputs, 1024 x 11008 x 4096 in 464 tiles of 128 x 192 (109 us; 126 in tiles of
-// 128, 136 in tiles of 256, 197 in tiles of 64), 1024 x 4096 x 4096 in 256 of 128 x 128 (44 us; 54 in tiles of 192), 67 x 190 x 10144 in 60 of 16 x 16 (8.5 us; 143 in
+// 128, 136 in tiles of 256, 197 in tiles of 64), 1024 x 4096 x 4096 in 256 of 128 x 128 (44 us; 54 in tiles of 192), 67 x 190 x 10144 in 204 of 4 x 16 (6.5 us; 143 in
 // tiles of 192).
 struct Form
 {
