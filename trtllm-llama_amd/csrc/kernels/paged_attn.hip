@@ -735,23 +735,11 @@ __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_p
     const int h = id % p.q_heads;
     id /= p.q_heads;
     const int i = id % per, b = id / per;
-    const Request req = request_of(p, b, shift);
-    const Split split = min(req.rows, p.max_new) * (p.q_heads / p.kv_heads) <= 16 ? light : heavy;
-    if (i >= req.rows || split.parts == 1)
-        return;
-    const int64_t at = split.at(b, req.row0, i, p.q_heads, h);
-    float m = -INFINITY, l = 0.f; // of part `lane`: there are 64 at most
-    if (lane < split.parts)
-    {
-        const float2 v = reinterpret_cast<const float2*>(split.ml)[at + lane];
-        m = v.x;
-        l = v.y;
-    }
-    const float m_all = wave_max(m), w = __builtin_amdgcn_exp2f(m - (m_all == -INFINITY ? 0.f : m_all)), sum = wave_sum(w * l);
-    float o[kPer] = {};
-    for (int s0 = 0; s0 < split.parts; s0 += 16) // four loads of a wave at a time
-    {
-        float x[4][kPer];
+    float2 ml = make_float2(-INFINITY, 0.f); // of part `lane`: there are 64 at most
+    float x[4][kPer] = {};                   // four parts of a wave at a time
+    auto send = [&](const Split& split, int64_t at, int s0) {
+        if (s0 == 0 && lane < split.parts)
+            ml = reinterpret_cast<const float2*>(split.ml)[at + lane];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
@@ -760,6 +748,28 @@ __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_p
             for (int e = 0; e < kPer; ++e)
                 x[k][e] = s < split.parts ? split.o[(at + s) * DIM + lane * kPer + e] : 0.f;
         }
+    };
+    // where the parts of a request of one tile lie does not hang on the request: they are sent for before it is known to be one
+    const int64_t at_light = light.at(b, 0, i, p.q_heads, h);
+    if (light.parts > 1 && i < light.per)
+        send(light, at_light, 0);
+    const Request req = request_of(p, b, shift);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+            asm volatile("" : "+v"(x[k][e])); // and not behind the branch
+    const bool few = min(req.rows, p.max_new) * (p.q_heads / p.kv_heads) <= 16;
+    const Split split = few ? light : heavy;
+    if (i >= req.rows || split.parts == 1)
+        return;
+    const int64_t at = few ? at_light : heavy.at(b, req.row0, i, p.q_heads, h);
+    if (!few)
+        send(heavy, at, 0);
+    const float m_all = wave_max(ml.x), w = __builtin_amdgcn_exp2f(ml.x - (m_all == -INFINITY ? 0.f : m_all)), sum = wave_sum(w * ml.y);
+    float o[kPer] = {};
+    for (int s0 = 0;;)
+    {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
@@ -768,6 +778,10 @@ __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_p
             for (int e = 0; e < kPer; ++e)
                 o[e] += ws * x[k][e];
         }
+        s0 += 16;
+        if (s0 >= split.parts)
+            break;
+        send(split, at, s0);
     }
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
