@@ -158,9 +158,9 @@ __global__ __launch_bounds__(DIM * kMaxPage / 32) void append_kernel(const tllm_
     const int page = 1 << shift, t0 = blockIdx.x * chunk, tid = threadIdx.x;
     const int kv_jobs = 2 * p.kv_heads;
     const bool pairs = p.rope_pairs != 0;
-    if ((int) blockIdx.y < kv_jobs && chunk > 1)
+    if ((int) blockIdx.y < kv_jobs)
     {
-        // most chunks of a prompt have no run's beginning: every wave sees that by itself (a row alone is no chunk: tokens would wait twice)
+        // most chunks of a prompt have no run's beginning: every wave sees that by itself
         bool any = false;
         for (int i = 0; i < chunk && !any; i += 63)
         {
