@@ -735,11 +735,11 @@ __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_p
     const int h = id % p.q_heads;
     id /= p.q_heads;
     const int i = id % per, b = id / per;
-    float2 ml = make_float2(-INFINITY, 0.f); // of part `lane`: there are 64 at most
+    float2 ml = make_float2(-INFINITY, 0.f); // of part `lane`: there are 64 at most; -INFINITY, 0: none
     float x[4][kPer] = {};                   // four parts of a wave at a time
     auto send = [&](const Split& split, int64_t at, int s0) {
-        if (s0 == 0 && lane < split.parts)
-            ml = reinterpret_cast<const float2*>(split.ml)[at + lane];
+        if (s0 == 0) // every lane: what one split has sent for is nothing of the other
+            ml = lane < split.parts ? reinterpret_cast<const float2*>(split.ml)[at + lane] : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
