@@ -256,4 +256,5 @@ class PagedKV8Cache(Fixed):
         need = lib.tllm_paged_attention_workspace(p)
         if need <= 0:  # none, or refused: the call says why
             return lib.tllm_paged_attention(p, None, stream)
-        return lib.tllm_paged_attention(p, torch.empty(need, dtype=torch.uint8, device=self.pool.device).data_ptr(), stream)
+        workspace = torch.empty(need, dtype=torch.uint8, device=self.pool.device)  # held over the call: another thread could be given it between the launches
+        return lib.tllm_paged_attention(p, workspace.data_ptr(), stream)
