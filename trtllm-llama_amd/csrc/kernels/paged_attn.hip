@@ -9,9 +9,11 @@
 //   P goes from the first product's registers into the second's as it is.  16 keys lie in one page, so a lane has one key scale and one value
 //   scale per tile.
 // 8-bit elements become fp16 exactly (int8: 0x6400 | (q + 128) = 1152 + q; e4m3: the convert instruction).  Scales enter in fp32: the key's with the
-// softmax scale behind the first product; the value's, relative to the largest value scale so far and times 2^7, in the exponent of the
-// weight.  m is brought along only when a score is more than 8 (a factor of 2^8) above it: a weight is at most 2^15, nothing overflows, it keeps
-// its 11 bits until its page's scale is 2^-21 of another's, and in most tiles no lane asks another for anything.
+// softmax scale behind the first product; the value's in the exponent of the weight, which is 2^7 times exp2(score) * scale over the largest such
+// product that the ROW has seen (its logarithm is mv, next to m for the sum).  What a row does not see, and what it does not weigh, does not enter its
+// mv: a page with values of 1e38 behind a row or outside its window costs the row nothing.  m and mv are brought along only when something is more
+// than 8 (a factor of 2^8) above them: a weight is at most 2^15, nothing overflows, it keeps its 11 bits until it is 2^-21 of the row's largest (where
+// 8-bit elements of the largest one's page are half a step, 2^-8 or 2^-10, off), and in most tiles no lane asks another for anything.
 //   rows_body   16 rows: four or eight waves take tiles in turn, straight from memory into registers, and join through LDS.  Single tokens are bound by the
 //               cache's bytes (48 requests over 4000 to 8000 keys, 8 key heads of 128, e4m3: 111 us, 5.4 TB/s); the keys are also split over workgroups,
 //               whose parts merge_kernel joins (131072 keys of one request: 42 + 4 us; a token over 1032, 32 heads: 7 + 4, the chain table -> keys ->
@@ -178,43 +180,20 @@ struct Split
     __device__ __forceinline__ int64_t at(int b, int row0, int i, int heads, int h) const { return ((int64_t) ((per ? b * per : row0) + i) * heads + h) * parts; }
 };
 
-// The value scales: the reference that O is in units of, and what a tile's pages say to a lane.
-struct Reference
+// What a row has seen: m, the largest score; mv, the largest score + log2 of its page's value scale; l, the sum of exp2(score - m).  O is in units of
+// exp2(mv - kPShift).
+struct Seen
 {
-    float v = 0.f, log_v = 0.f;
+    float m = -INFINITY, mv = -INFINITY, l = 0.f;
+    __device__ __forceinline__ float unit() const { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - m - kPShift); } // of O, in units of l
 };
-struct TileScales
-{
-    float ks, vs;
-    float lift, drop; // weights are formed times 2^lift; 2^-lift
-    float back;       // what O has to be multiplied by as the reference grows
-};
-__device__ __forceinline__ TileScales scales_of(float ks, float vs, Reference& ref)
-{
-    TileScales t;
-    t.ks = ks;
-    t.vs = vs;
-    t.back = 1.f;
-    if (__builtin_amdgcn_ballot_w64(vs > ref.v))
-    {
-        const float v_new = fmaxf(ref.v, groups_max(vs));
-        t.back = ref.v / v_new;
-        ref.v = v_new;
-        ref.log_v = __builtin_amdgcn_logf(v_new);
-    }
-    // below 2^-60 of the reference a page's weights are 0 in fp16 either way; l still has to see them
-    t.lift = fmaxf(__builtin_amdgcn_logf(vs) - ref.log_v + kPShift, -60.f);
-    t.drop = __builtin_amdgcn_exp2f(-t.lift);
-    return t;
-}
 
-// One tile of one row: the 16 scores of a lane (keys key0 .. + 15 of a query's row) -> its weights in fp16, with m, l and O brought along.  `plain`
-// (the same for the wave): every key is seen.
+// One tile of one row: the 16 scores of a lane (keys key0 .. + 15 of a query's row), under the key scale `ks` of their page and log2 of its value scale `lv` -> its weights in fp16, with what
+// the row has seen and O brought along.  `plain` (the same for the wave): every key is seen.
 template <int N>
-__device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], float& m, float& l, f32x4 (&o)[N], const TileScales& t, float factor, bool plain, bool in, int key0,
-    int from, int seen)
+__device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], Seen& r, f32x4 (&o)[N], float ks, float lv, float factor, bool plain, bool in, int key0, int from, int seen)
 {
-    float f = factor * t.ks;
+    float f = factor * ks;
     if (!plain)
     {
 #pragma unroll
@@ -227,27 +206,30 @@ __device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], float& m, 
     for (int i = 1; i < 16; ++i)
         top = fmaxf(top, s[i]);
     top *= f; // f >= 0
-    if (__builtin_amdgcn_ballot_w64(top > m + kSlack || t.back != 1.f))
+    const float top_v = top + lv;
+    if (__builtin_amdgcn_ballot_w64(top > r.m + kSlack || top_v > r.mv + kSlack))
     {
-        const float m_new = fmaxf(m, groups_max(top));
-        const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new), back = alpha * t.back;
-        l *= alpha;
-        m = m_new;
+        const float m = fmaxf(r.m, groups_max(top)), mv = fmaxf(r.mv, groups_max(top_v));
+        const float back = mv == r.mv ? 1.f : __builtin_amdgcn_exp2f(r.mv - mv);
+        r.l *= m == r.m ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+        r.m = m;
+        r.mv = mv;
 #pragma unroll
         for (int i = 0; i < N; ++i)
             o[i] *= back;
     }
-    const float shift = t.lift - (m == -INFINITY ? 0.f : m);
+    // weights are exp2(score + lift).  Where that would be below 2^-60 they are 0 in fp16 either way, and only l has to see them
+    const float m = r.m == -INFINITY ? 0.f : r.m, lift = fmaxf(lv - (r.mv == -INFINITY ? 0.f : r.mv), -60.f - m) + kPShift;
     float sum = 0.f;
     u32x4 p[2];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
     {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], f, shift)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], f, shift));
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], f, lift)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], f, lift));
         sum += a + b;
         p[i >> 2][i & 3] = pack_f16(a, b);
     }
-    l += sum * t.drop;
+    r.l += sum * __builtin_amdgcn_exp2f(-lift - m);
     w[0] = join(p[0]);
     w[1] = join(p[1]);
 }
@@ -333,8 +315,7 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
 #pragma unroll
     for (int i = 0; i < kOut; ++i)
         o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    Reference ref;
+    Seen row_seen;
     // The last tile of a wave sends for nothing.  It is a body of its own: with the loads under a condition inside one loop the compiler's scheduler
     // has written over registers of the values that were still to be read (hipcc 7.2, seen in the assembly and by the tests).
     auto step = [&](int t, auto more) {
@@ -363,10 +344,9 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
             if (t + 2 * NW < t_end)
                 blocks_of(t + 2 * NW);
         }
-        const TileScales scales = scales_of(ks, vs, ref);
         const int keep = v_in ? req.len - vk : 0;
         f16x8 w[2];
-        soften(s, w, m, l, o, scales, factor, __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen || vk < from) == 0, v_in, vk, from, seen);
+        soften(s, w, row_seen, o, ks, __builtin_amdgcn_logf(vs), factor, __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen || vk < from) == 0, v_in, vk, from, seen);
         if (__builtin_amdgcn_ballot_w64(keep < 16))
 #pragma unroll
             for (int i = 0; i < kOut; ++i)
@@ -390,7 +370,7 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
     }
 
     // the waves' parts -> one
-    l = groups_sum(l);
+    const float m = row_seen.m, l = groups_sum(row_seen.l);
     if (g == 0)
     {
         ms[wave][r] = m;
@@ -401,7 +381,7 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
 #pragma unroll
     for (int w = 1; w < NW; ++w)
         m_all = fmaxf(m_all, ms[w][r]);
-    const float mine = __builtin_amdgcn_exp2f(m - (m_all == -INFINITY ? 0.f : m_all)) * (ref.v * __builtin_amdgcn_exp2f(-kPShift));
+    const float mine = m_all == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(row_seen.mv - m_all - kPShift);
     if (wave >= kPlaces)
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
@@ -573,8 +553,8 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
 
     f16x8 q[RT][kSteps];
     f32x4 o[RT][kOut];
-    float factor[RT], m[RT], l[RT];
-    Reference ref;
+    float factor[RT];
+    Seen rows_seen[RT];
     int seen[RT], from[RT];
     if (t_begin < t_end)
     {
@@ -592,8 +572,6 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
         factor[i] = load_query<DIM, BF16>(q[i], q_row, g) * p.scale * kLog2e;
         seen[i] = live ? first + token + 1 : 0x7fffffff;
         from[i] = live && p.window > 0 ? seen[i] - p.window : 0;
-        m[i] = -INFINITY;
-        l[i] = 0.f;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
             o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -654,11 +632,11 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
 #pragma unroll
             for (int j = 0; j < kAhead; ++j)
                 a[0][j] = vt[j * 64];
-            const TileScales scales = scales_of(ks, vs, ref);
+            const float lv = __builtin_amdgcn_logf(vs);
             f16x8 w[RT][2];
 #pragma unroll
             for (int n = 0; n < RT; ++n)
-                soften(s[n], w[n], m[n], l[n], o[n], scales, factor[n], __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen[n] || vk < from[n]) == 0, v_in, vk, from[n], seen[n]);
+                soften(s[n], w[n], rows_seen[n], o[n], ks, lv, factor[n], __builtin_amdgcn_ballot_w64(!v_in || vk + 16 > seen[n] || vk < from[n]) == 0, v_in, vk, from[n], seen[n]);
 #pragma unroll
             for (int i = 0; i < F::kKeyFrags / kAhead; ++i) // as many fragments of values: channels 16 (f / 2), keys 32 (f % 2)
             {
@@ -698,11 +676,11 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
 #pragma unroll
     for (int n = 0; n < RT; ++n)
     {
-        const float sum = groups_sum(l[n]);
+        const float sum = groups_sum(rows_seen[n].l);
         const int row = my0 + 16 * n + r, token = row / group, qh = head * group + row - token * group;
         if (row >= rows)
             continue;
-        const float unit = ref.v * __builtin_amdgcn_exp2f(-kPShift);
+        const float unit = rows_seen[n].unit();
         if (split.parts > 1)
         {
             const int64_t at = split.at(b, req.row0, token, p.q_heads, qh) + part;
@@ -711,7 +689,7 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
                 *reinterpret_cast<f32x4*>(split.o + at * DIM + 16 * d + 4 * g) = o[n][d] * unit;
             if (g == 0)
             {
-                split.ml[2 * at] = m[n];
+                split.ml[2 * at] = rows_seen[n].m;
                 split.ml[2 * at + 1] = sum;
             }
             continue;
