@@ -80,3 +80,18 @@ def test_a_far_page_without_weight_takes_nothing(lens, rows, max_kv, size):
     cache.scales[at, 1] = 2.0**40
     q = torch.from_numpy(rng.uniform(0.5, 1, (sum(rows), 2, size)).astype(np.float32)).bfloat16()  # scores of -100 and less
     assert (np.abs(check(cache, q, 'bf16', lens, rows, max_kv=max_kv)) < 3).all()
+
+
+@pytest.mark.parametrize('size', [64, 128, 256])
+@pytest.mark.parametrize('lens,rows,max_kv', [([40], [1], None)] + SPANS)
+def test_the_largest_values_stay_finite(lens, rows, max_kv, size):
+    """Every value the largest that the cache gives bfloat16 (infinities count as it), then half of them its negative: the mean is exact but for the weights'
+    rounding, and far from the type's end or within half a step of it."""
+    rng = np.random.default_rng(size + 2)
+    cache = cache_of(rng, sum(-(-n // PAGE) for n in lens), size)
+    largest = float(torch.finfo(torch.bfloat16).max)
+    cache.scales[:, 1] = largest / 127
+    q = torch.zeros((sum(rows), 2, size), dtype=torch.bfloat16)
+    for values in (torch.full((PAGE, ), 127), torch.tensor([127, -127] * (PAGE // 2))):
+        cache.pool[:, 1] = values.to(torch.int8).cuda().repeat(size)
+        check(cache, q, 'bf16', lens, rows, max_kv=max_kv)

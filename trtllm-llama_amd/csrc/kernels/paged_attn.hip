@@ -173,20 +173,27 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b)
 // The keys of a row in parts, each by its own workgroup.
 struct Split
 {
-    float* o;  // [rows][q_heads][parts][DIM], not divided by l
-    float* ml; // [rows][q_heads][parts][2]
+    float* o;     // [rows][q_heads][parts][DIM], not divided by l
+    float4* seen; // [rows][q_heads][parts]: m, l, mv
     int parts;
     int per; // rows a request has in these, 0: they are the batch's rows
     __device__ __forceinline__ int64_t at(int b, int row0, int i, int heads, int h) const { return ((int64_t) ((per ? b * per : row0) + i) * heads + h) * parts; }
 };
 
 // What a row has seen: m, the largest score; mv, the largest score + log2 of its page's value scale; l, the sum of exp2(score - m).  O is in units of
-// exp2(mv - kPShift).
+// exp2(mv - kPShift) until it is stored as the result: what l times the largest bfloat16 value is has no place in fp32.
 struct Seen
 {
     float m = -INFINITY, mv = -INFINITY, l = 0.f;
-    __device__ __forceinline__ float unit() const { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - m - kPShift); } // of O, in units of l
 };
+__device__ __forceinline__ float part_of(float mine, float all) // exp2(mine - all), where a part or all of them may have seen nothing
+{
+    return all == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - all);
+}
+__device__ __forceinline__ float result_of(float m, float mv, float l) // of O; a row that saw nothing is 0, a NaN stays one
+{
+    return (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) * part_of(mv - kPShift, m);
+}
 
 // One tile of one row: the 16 scores of a lane (keys key0 .. + 15 of a query's row), under the key scale `ks` of their page and log2 of its value scale `lv` -> its weights in fp16, with what
 // the row has seen and O brought along.  `plain` (the same for the wave): every key is seen.
@@ -238,7 +245,7 @@ template <int DIM, int NW>
 struct RowsLds
 {
     static constexpr int kLine = DIM + 4;
-    static constexpr int kBytes = (NW / 2 * 16 * kLine + NW * 32) * 4;
+    static constexpr int kBytes = (NW / 2 * 16 * kLine + NW * 48) * 4;
 };
 
 // 16 rows (`tile`) of a request and key head, keys of one part
@@ -250,6 +257,7 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
     float(*acc)[16][kLine] = reinterpret_cast<float(*)[16][kLine]>(lds);
     float(*ms)[16] = reinterpret_cast<float(*)[16]>(lds + kPlaces * 16 * kLine);
     float(*ls)[16] = ms + NW;
+    float(*mvs)[16] = ls + NW;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
     const int group = p.q_heads / p.kv_heads;
     const int rows = min(req.rows, p.max_new) * group, row = tile * 16 + r;
@@ -370,18 +378,19 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
     }
 
     // the waves' parts -> one
-    const float m = row_seen.m, l = groups_sum(row_seen.l);
+    const float l = groups_sum(row_seen.l);
     if (g == 0)
     {
-        ms[wave][r] = m;
+        ms[wave][r] = row_seen.m;
         ls[wave][r] = l;
+        mvs[wave][r] = row_seen.mv;
     }
     __syncthreads();
-    float m_all = ms[0][r];
+    float mv_all = mvs[0][r];
 #pragma unroll
     for (int w = 1; w < NW; ++w)
-        m_all = fmaxf(m_all, ms[w][r]);
-    const float mine = m_all == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(row_seen.mv - m_all - kPShift);
+        mv_all = fmaxf(mv_all, mvs[w][r]);
+    const float mine = part_of(row_seen.mv, mv_all);
     if (wave >= kPlaces)
 #pragma unroll
         for (int i = 0; i < kOut; ++i)
@@ -400,15 +409,17 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
         const int ur = u / (DIM / 4), d = u % (DIM / 4) * 4, urow = tile * 16 + ur;
         if (urow >= rows)
             continue;
-        float um = ms[0][ur];
+        float um = ms[0][ur], umv = mvs[0][ur];
 #pragma unroll
         for (int w = 1; w < NW; ++w)
+        {
             um = fmaxf(um, ms[w][ur]);
-        const float uu = um == -INFINITY ? 0.f : um;
+            umv = fmaxf(umv, mvs[w][ur]);
+        }
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w)
-            sum += ls[w][ur] * __builtin_amdgcn_exp2f(ms[w][ur] - uu);
+            sum += ls[w][ur] * __builtin_amdgcn_exp2f(ms[w][ur] - (um == -INFINITY ? 0.f : um));
         f32x4 a = *reinterpret_cast<const f32x4*>(&acc[0][ur][d]);
 #pragma unroll
         for (int i = 1; i < kPlaces; ++i)
@@ -419,15 +430,12 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
             const int64_t at = split.at(b, req.row0, utoken, p.q_heads, uh) + part;
             *reinterpret_cast<f32x4*>(split.o + at * DIM + d) = a;
             if (d == 0)
-            {
-                split.ml[2 * at] = um;
-                split.ml[2 * at + 1] = sum;
-            }
+                split.seen[at] = make_float4(um, sum, umv, 0.f);
             continue;
         }
-        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); // a row that saw nothing is 0, a NaN stays one
+        const float to = result_of(um, umv, sum);
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (req.row0 + utoken) * p.out_row + uh * p.out_head + d)
-            = make_uint2(pack_out<BF16>(a[0] * inv, a[1] * inv), pack_out<BF16>(a[2] * inv, a[3] * inv));
+            = make_uint2(pack_out<BF16>(a[0] * to, a[1] * to), pack_out<BF16>(a[2] * to, a[3] * to));
     }
 }
 
@@ -680,25 +688,21 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
         const int row = my0 + 16 * n + r, token = row / group, qh = head * group + row - token * group;
         if (row >= rows)
             continue;
-        const float unit = rows_seen[n].unit();
         if (split.parts > 1)
         {
             const int64_t at = split.at(b, req.row0, token, p.q_heads, qh) + part;
 #pragma unroll
             for (int d = 0; d < kOut; ++d)
-                *reinterpret_cast<f32x4*>(split.o + at * DIM + 16 * d + 4 * g) = o[n][d] * unit;
+                *reinterpret_cast<f32x4*>(split.o + at * DIM + 16 * d + 4 * g) = o[n][d];
             if (g == 0)
-            {
-                split.ml[2 * at] = rows_seen[n].m;
-                split.ml[2 * at + 1] = sum;
-            }
+                split.seen[at] = make_float4(rows_seen[n].m, sum, rows_seen[n].mv, 0.f);
             continue;
         }
-        const float inv = (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) * unit;
+        const float by = result_of(rows_seen[n].m, rows_seen[n].mv, sum);
         uint16_t* const to = static_cast<uint16_t*>(p.out) + (req.row0 + token) * p.out_row + qh * p.out_head + 4 * g;
 #pragma unroll
         for (int d = 0; d < kOut; ++d)
-            *reinterpret_cast<uint2*>(to + 16 * d) = make_uint2(pack_out<BF16>(o[n][d][0] * inv, o[n][d][1] * inv), pack_out<BF16>(o[n][d][2] * inv, o[n][d][3] * inv));
+            *reinterpret_cast<uint2*>(to + 16 * d) = make_uint2(pack_out<BF16>(o[n][d][0] * by, o[n][d][1] * by), pack_out<BF16>(o[n][d][2] * by, o[n][d][3] * by));
     }
 }
 
@@ -713,11 +717,11 @@ __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_p
     const int h = id % p.q_heads;
     id /= p.q_heads;
     const int i = id % per, b = id / per;
-    float2 ml = make_float2(-INFINITY, 0.f); // of part `lane`: there are 64 at most; -INFINITY, 0: none
-    float x[4][kPer] = {};                   // four parts of a wave at a time
+    float4 seen;           // of part `lane`: there are 64 at most
+    float x[4][kPer] = {}; // four parts of a wave at a time
     auto send = [&](const Split& split, int64_t at, int s0) {
         if (s0 == 0) // every lane: what one split has sent for is nothing of the other
-            ml = lane < split.parts ? reinterpret_cast<const float2*>(split.ml)[at + lane] : make_float2(-INFINITY, 0.f);
+            seen = lane < split.parts ? split.seen[at + lane] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
@@ -744,7 +748,8 @@ __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_p
     const int64_t at = few ? at_light : heavy.at(b, req.row0, i, p.q_heads, h);
     if (!few)
         send(heavy, at, 0);
-    const float m_all = wave_max(ml.x), w = __builtin_amdgcn_exp2f(ml.x - (m_all == -INFINITY ? 0.f : m_all)), sum = wave_sum(w * ml.y);
+    const float m = wave_max(seen.x), mv = wave_max(seen.z), w = part_of(seen.z, mv);
+    const float by = result_of(m, mv, wave_sum(seen.y * __builtin_amdgcn_exp2f(seen.x - (m == -INFINITY ? 0.f : m))));
     float o[kPer] = {};
     for (int s0 = 0;;)
     {
@@ -765,10 +770,9 @@ __global__ __launch_bounds__(256) void merge_kernel(const tllm_paged_attention_p
     for (int e = 0; e < kPer; ++e)
         os[wave][lane * kPer + e] = o[e];
     __syncthreads();
-    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
     for (int d = threadIdx.x; d < DIM; d += 256)
     {
-        const float v = (os[0][d] + os[1][d] + os[2][d] + os[3][d]) * inv;
+        const float v = (os[0][d] + os[1][d] + os[2][d] + os[3][d]) * by;
         static_cast<uint16_t*>(p.out)[(req.row0 + i) * p.out_row + h * p.out_head + d] = BF16 ? f2bf(v) : f2h(v);
     }
 }
@@ -838,8 +842,8 @@ void launch_form(const tllm_paged_attention_params_t& p, void* workspace, hipStr
     const Parts s = parts_of(p);
     const auto n = places_of(p, s);
     float* const o = static_cast<float*>(workspace);
-    float* const ml = o + (n.light + n.heavy) * DIM;
-    const Split light = {o, ml, s.light, s.per}, heavy = {o + n.light * DIM, ml + n.light * 2, s.heavy, 0};
+    float4* const seen = reinterpret_cast<float4*>(o + (n.light + n.heavy) * DIM);
+    const Split light = {o, seen, s.light, s.per}, heavy = {o + n.light * DIM, seen + n.light, s.heavy, 0};
     if (one_tile(p))
     {
         if constexpr (DIM < 256)
@@ -876,7 +880,7 @@ void launch_dim(const tllm_paged_attention_params_t& p, void* workspace, hipStre
 size_t paged_attention_workspace(const tllm_paged_attention_params_t& p)
 {
     const Places n = places_of(p, parts_of(p));
-    return (size_t) (n.light + n.heavy) * (p.head_size + 2) * 4;
+    return (size_t) (n.light + n.heavy) * (p.head_size + 4) * 4;
 }
 
 int launch_paged_attention(const tllm_paged_attention_params_t& p, void* workspace, hipStream_t stream)
