@@ -95,3 +95,15 @@ def test_the_largest_values_stay_finite(lens, rows, max_kv, size):
     for values in (torch.full((PAGE, ), 127), torch.tensor([127, -127] * (PAGE // 2))):
         cache.pool[:, 1] = values.to(torch.int8).cuda().repeat(size)
         check(cache, q, 'bf16', lens, rows, max_kv=max_kv)
+
+
+@pytest.mark.parametrize('size', [64, 128, 256])
+@pytest.mark.parametrize('lens,rows,max_kv', SPANS)
+def test_keys_of_nothing_in_a_page_of_the_largest(lens, rows, max_kv, size):
+    """Keys that are zero under the largest scale score zero, however large the query."""
+    rng = np.random.default_rng(size + 3)
+    cache = cache_of(rng, sum(-(-n // PAGE) for n in lens), size)
+    cache.pool[:, 0] = 0
+    cache.scales[:, 0] = float(torch.finfo(torch.bfloat16).max) / 127
+    q = torch.from_numpy(rng.standard_normal((sum(rows), 2, size)).astype(np.float32) * 2.0**20).bfloat16()
+    check(cache, q, 'bf16', lens, rows, max_kv=max_kv)

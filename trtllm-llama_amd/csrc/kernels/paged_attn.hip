@@ -200,7 +200,7 @@ __device__ __forceinline__ float result_of(float m, float mv, float l) // of O; 
 template <int N>
 __device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], Seen& r, f32x4 (&o)[N], float ks, float lv, float factor, bool plain, bool in, int key0, int from, int seen)
 {
-    float f = factor * ks;
+    float f = fminf(factor * ks, 3.4028235e38f); // zero keys under the largest scale score 0, not 0 times an infinity
     if (!plain)
     {
 #pragma unroll
