@@ -107,6 +107,8 @@ int32_t tllm_paged_append(const tllm_paged_append_params_t* p, tllm_stream_t str
  *   max_kv   an expectation of the longest kv_lens, for how the work is split; any kv_lens up to max_blocks * page_size is right.
  * Table entries that are no block of the pool count as masked.  Lengths beyond the table are cut to it.
  * out may be q itself, with its strides.
+ * At most 4096 requests and 2^19 rows; n_seqs * kv_heads * ceil(max_new * (q_heads / kv_heads) / 128) is at most 2^25 (64 for 128 with heads of 256): the work is
+ * laid out as if every request had max_new rows, and what none has costs a workgroup's start.
  * Workspace: tllm_paged_attention_workspace() bytes, 16-byte aligned, not shared by calls that may overlap.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct

@@ -478,11 +478,14 @@ __global__ __launch_bounds__(256, DIM == 64 ? 3 : 2) void tile_kernel(const tllm
     // the last ones to begin are short (12 requests of up to 700, 32 heads of 128: 117 us, 125 pair after pair; 4 of 1024 behind 3000, 32 heads on 8: 223, 234).  Where
     // every tile has a place from the start, the second half comes the other way round: workgroups 32 apart of an XCD meet on one CU, a light one
     // beside a heavy one (2048 tokens behind 1500, 32 heads of 128: 114 us, 116 without, 126 pair after pair; heads of 64: 79, 82, 91).
-    const int id = blockIdx.x - light_groups, xcd = id & 7, pairs8 = (p.n_seqs * p.kv_heads + 7) >> 3, mine = pairs8 * row_tiles;
+    const int group_id = blockIdx.z * gridDim.x + blockIdx.x; // a launch of many workgroups goes on in z
+    const int id = group_id - light_groups, xcd = id & 7, pairs8 = (p.n_seqs * p.kv_heads + 7) >> 3, mine = pairs8 * row_tiles;
+    if (id >= 8 * mine)
+        return;
     const int at8 = mine <= 64 && id >> 3 >= 32 ? 32 + mine - 1 - (id >> 3) : id >> 3;
     const int most = max(1, 64 / row_tiles), turn = at8 / (most * row_tiles), in = at8 - turn * (most * row_tiles), width = min(most, pairs8 - turn * most);
     const int tile = id < 0 ? 0 : row_tiles - 1 - in / width;
-    const int part = id < 0 ? blockIdx.x % light.parts : blockIdx.y, pair = id < 0 ? blockIdx.x / light.parts : (turn * most + in % width) * 8 + xcd;
+    const int part = id < 0 ? group_id % light.parts : blockIdx.y, pair = id < 0 ? group_id / light.parts : (turn * most + in % width) * 8 + xcd;
     if (pair >= p.n_seqs * p.kv_heads)
         return;
     const int head = pair % p.kv_heads, b = pair / p.kv_heads, group = p.q_heads / p.kv_heads;
@@ -859,8 +862,8 @@ void launch_form(const tllm_paged_attention_params_t& p, void* workspace, hipStr
         using F = TileForm<DIM>;
         const int row_tiles = row_tiles_of(p), light_groups = s.light > 1 ? (int) ((pairs * s.light + 7) / 8 * 8) : 0;
         launch_util::ensure_dynamic_lds(reinterpret_cast<const void*>(&tile_kernel<DIM, BF16, FP8>), F::kLds);
-        tile_kernel<DIM, BF16, FP8>
-            <<<dim3((unsigned) (light_groups + (pairs + 7) / 8 * 8 * row_tiles), s.heavy), 256, F::kLds, stream>>>(p, shift, row_tiles, light_groups, light, heavy);
+        const int64_t all = light_groups + (pairs + 7) / 8 * 8 * row_tiles, wide = std::min<int64_t>(all, 1 << 22); // both multiples of 8; 2^32 threads are too many in x
+        tile_kernel<DIM, BF16, FP8><<<dim3((unsigned) wide, s.heavy, (unsigned) ((all + wide - 1) / wide)), 256, F::kLds, stream>>>(p, shift, row_tiles, light_groups, light, heavy);
     }
     const int per = s.heavy > 1 ? p.max_new : s.per;
     if (s.light > 1 || s.heavy > 1)

@@ -37,7 +37,7 @@ bool overlap(const Range& a, const Range& b)
     return a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
 }
 
-constexpr int32_t kMaxRows = 1 << 19, kMaxHeads = 1024;
+constexpr int32_t kMaxRows = 1 << 19, kMaxHeads = 1024, kMaxTiles = 1 << 25;
 
 #define TLLM_REFUSE(cond, ...)                                                                                         \
     do                                                                                                                 \
@@ -136,10 +136,10 @@ bool attention_fits(const tllm_paged_attention_params_t* p)
     TLLM_REFUSE(!(p->scale >= 0.f && p->scale < 1e30f), "%s: the scale is negative or not finite", me);
     TLLM_REFUSE(!p->block_table || !p->cu_tokens || !p->kv_lens || !aligned(p->block_table, 4) || !aligned(p->cu_tokens, 4) || !aligned(p->kv_lens, 4),
         "%s: tables and lengths are null or not 4-byte aligned", me);
-    const int64_t max_new = std::min(p->max_new, p->n_rows);
-    TLLM_REFUSE((int64_t) p->n_seqs * p->kv_heads * ((max_new * (p->q_heads / p->kv_heads) + 15) / 16) > INT32_MAX / 64 - 8
-            || p->n_seqs * max_new * p->q_heads > INT32_MAX,
-        "%s: %d requests of up to %lld rows are more than one launch takes", me, p->n_seqs, (long long) max_new);
+    // what does not go into one launch: row tiles of every request and key head, as many as one request may have
+    const int64_t rows = (int64_t) std::min(p->max_new, p->n_rows) * (p->q_heads / p->kv_heads), in_tile = p->head_size == 256 ? 64 : 128;
+    TLLM_REFUSE((int64_t) p->n_seqs * p->kv_heads * ((rows + in_tile - 1) / in_tile) > kMaxTiles, "%s: %d requests of up to %d rows are more than one launch takes", me, p->n_seqs,
+        p->max_new);
     return p->n_rows == 0 || (rows_fit(me, "q", p->q, p->q_row, p->q_head) && rows_fit(me, "out", p->out, p->out_row, p->out_head));
 }
 
