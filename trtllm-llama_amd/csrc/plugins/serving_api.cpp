@@ -25,16 +25,55 @@ bool aligned(const void* p, size_t to)
     return reinterpret_cast<uintptr_t>(p) % to == 0;
 }
 
+// `rows` pieces of `bytes`, one every `step` bytes
 struct Range
 {
-    const void* at;
-    int64_t bytes;
+    int64_t at, bytes, rows, step;
+    Range(const void* p, int64_t bytes, int64_t rows = 1, int64_t step = 0)
+        : at(static_cast<int64_t>(reinterpret_cast<uintptr_t>(p))), bytes(bytes), rows(bytes > 0 ? rows : 0), step(step)
+    {
+        if (rows > 1 && step < 0)
+        {
+            at += (rows - 1) * step;
+            this->step = -step;
+        }
+        if (rows > 1 && this->step == bytes)
+        {
+            this->bytes *= rows;
+            this->rows = 1;
+        }
+        if (this->rows <= 1)
+            this->step = 0;
+    }
+    int64_t end() const { return at + (rows - 1) * step + bytes; }
+    bool operator==(const Range& o) const { return at == o.at && bytes == o.bytes && rows == o.rows && step == o.step; }
 };
+
+int64_t floor_div(int64_t a, int64_t b)
+{
+    return a / b - (a % b < 0);
+}
+
+// a piece at `at` + k * step, first <= k <= last, reaches into [x, x + n)
+bool meets(int64_t at, int64_t bytes, int64_t step, int64_t first, int64_t last, int64_t x, int64_t n)
+{
+    if (step == 0)
+        return at < x + n && x < at + bytes;
+    return std::max(first, floor_div(x - bytes - at, step) + 1) <= std::min(last, -floor_div(at - x - n, step) - 1);
+}
 
 bool overlap(const Range& a, const Range& b)
 {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
-    return a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+    if (a.rows <= 0 || b.rows <= 0 || a.at >= b.end() || b.at >= a.end())
+        return false;
+    if (a.rows > b.rows)
+        return overlap(b, a);
+    if (a.step == b.step) // only the distance counts
+        return meets(b.at, b.bytes, b.step, 1 - a.rows, b.rows - 1, a.at, a.bytes);
+    for (int64_t i = 0; i < a.rows; ++i)
+        if (meets(b.at, b.bytes, b.step, 0, b.rows - 1, a.at + i * a.step, a.bytes))
+            return true;
+    return false;
 }
 
 constexpr int32_t kMaxRows = 1 << 19, kMaxHeads = 1024, kMaxTiles = 1 << 25;
@@ -67,15 +106,17 @@ bool plan_fits(const tllm_paged_plan_params_t* p)
         TLLM_REFUSE(!aligned(t, 4), "%s: a tensor is not 4-byte aligned", me);
     // several workgroups read what one of them writes, unless it is the whole of the same state
     const int64_t n = p->n_seqs * 4, rows = p->n_rows * 4;
-    const Range reads[] = {{p->lens, n}, {p->new_lens, n}, {p->ring_state, 8}, {p->ring, (int64_t) p->num_blocks * 4}};
-    const Range writes[] = {{p->lens_out, n}, {p->ring_state_out, 8}, {p->cu_tokens, n + 4}, {p->slot_map, rows}, {p->positions, rows}, {p->status, 4}};
+    const Range lens(p->lens, n), state(p->ring_state, 8), lens_out(p->lens_out, n), state_out(p->ring_state_out, 8);
+    const Range reads[] = {lens, {p->new_lens, n}, state};
+    const Range writes[] = {lens_out, state_out, {p->cu_tokens, n + 4}, {p->slot_map, rows}, {p->positions, rows}, {p->status, 4}, {p->ring, (int64_t) p->num_blocks * 4},
+        {p->block_table, (int64_t) p->max_blocks * 4, p->n_seqs, p->table_stride * 4}};
     for (const Range& w : writes)
     {
         for (const Range& r : reads)
-            TLLM_REFUSE(overlap(w, r) && !(w.at == r.at && ((w.at == p->lens_out && r.at == p->lens) || (w.at == p->ring_state_out && r.at == p->ring_state))),
+            TLLM_REFUSE(overlap(w, r) && !((&w == &writes[0] && &r == &reads[0] && w == r) || (&w == &writes[1] && &r == &reads[2] && w == r)),
                 "%s: a result lies where another tensor does", me);
         for (const Range& o : writes)
-            TLLM_REFUSE(&o != &w && overlap(w, o), "%s: a result lies where another tensor does", me);
+            TLLM_REFUSE(&o < &w && overlap(w, o), "%s: a result lies where another tensor does", me);
     }
     return true;
 }
