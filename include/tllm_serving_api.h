@@ -138,7 +138,7 @@ int32_t tllm_paged_attention(const tllm_paged_attention_params_t* p, void* works
  *   packed  [ceil(N / 16)][ceil(K / 128)][64][16] bytes: lane l = 16 g + r of a tile holds, in its 32-bit word j, row r's eight
  *           elements k = 32 j + 8 g + e of the tile, as nibbles q + 8 in the order e = 0 2 4 6 1 3 5 7; padding is 8 (zero);
  *   scales  [ceil(K / group)][16 * ceil(N / 16)], padding 0.
- * x rows start 16-byte aligned (ldx a multiple of 8); y rows 2-byte aligned; y does not overlap x.
+ * x rows start 16-byte aligned (ldx a multiple of 8); y rows 2-byte aligned; no row of y lies on one of x or on the weights (rows of both may alternate).
  * ---------------------------------------------------------------------------------------------- */
 typedef struct
 {

@@ -5,8 +5,9 @@ import pytest
 import torch
 
 from tensorrt_llm.plugin import capi
+from tensorrt_llm.quantization import group as G
 from tensorrt_llm.runtime import paged_kv8 as P
-from test_serving_api_host import AT, plan_params
+from test_serving_api_host import AT, MatmulParams, plan_params
 
 # a call that passes the checks ends at the launch, which there has to be no device for: its addresses are made up
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason='the addresses are no memory')
@@ -48,3 +49,30 @@ def test_plan_finds_every_place_in_a_table(stride):
     for word in range(-8, p.n_seqs * stride + 8):
         lens = {base + 4 * (word + i) for i in range(p.n_seqs)}
         assert refused(lambda q: P._lib().tllm_paged_plan(ctypes.addressof(q), None), p, 'lies where', new_lens=base + 4 * word) == bool(lens & table), word
+
+
+def matmul(**with_):
+    p = MatmulParams(8, 24, 64, 32, capi.HALF, 64, 24, AT, 4 * AT, 5 * AT, 2 * AT)
+    for k, v in with_.items():
+        setattr(p, k, v)
+    return G._entry()(ctypes.addressof(p), None) != 0 and 'y lies' in capi.last_error()
+
+
+def test_products_refuse_results_on_their_operands():
+    assert not matmul()
+    assert matmul(y=AT) and matmul(y=AT + 2 * 64 * 8 - 2) and not matmul(y=AT + 2 * 64 * 8) and matmul(y=AT - 2 * 24 * 8 + 2) and not matmul(y=AT - 2 * 24 * 8)
+    assert matmul(y=4 * AT + 2) and matmul(y=5 * AT + 2 * 32 * 2 - 2) and not matmul(y=5 * AT + 2 * 32 * 2)  # 2 tiles of 16 outputs, one k-tile; 2 groups of 32 scales
+    # rows of one buffer: y behind x, y before x, y across x
+    for ld in (88, 96, 200):
+        assert not matmul(ldx=ld, ldy=ld, y=AT + 128) and not matmul(ldx=ld, ldy=ld, y=AT - 48)
+        assert matmul(ldx=ld, ldy=ld, y=AT + 126) and matmul(ldx=ld, ldy=ld, y=AT - 46)
+        assert matmul(ldx=ld, ldy=ld, y=AT + 128 + 14 * ld) is False and matmul(ldx=ld, ldy=ld, y=AT + 126 + 14 * ld)  # seven rows on
+    assert matmul(rows=1, y=AT + 126) and not matmul(rows=1, y=AT + 128)
+
+
+def test_products_of_rows_of_any_two_strides_against_sets_of_places():
+    for ldx, ldy, rows in ((64, 24, 5), (72, 40, 6), (128, 136, 4), (200, 24, 3)):
+        x = {2 * (r * ldx + c) for r in range(rows) for c in range(64)}
+        for first in range(-2 * rows * ldy - 64, 2 * rows * ldx + 64, 10):
+            y = {first + 2 * (r * ldy + c) for r in range(rows) for c in range(24)}
+            assert matmul(rows=rows, ldx=ldx, ldy=ldy, y=AT + first) == bool(x & y), (ldx, ldy, first)

@@ -195,7 +195,13 @@ bool matmul_fits(const tllm_group_matmul_params_t* p)
     TLLM_REFUSE(!p->packed || !aligned(p->packed, 16) || !p->scales || !aligned(p->scales, 16), "%s: weights or scales are null or not 16-byte aligned", me);
     TLLM_REFUSE(p->rows && (!p->x || !aligned(p->x, 16) || p->ldx % 8 || (p->rows > 1 && p->ldx < p->k)), "%s: x has to be 16-byte aligned with a row stride that is a multiple of 8, at least k", me);
     TLLM_REFUSE(p->rows && (!p->y || !aligned(p->y, 2) || (p->rows > 1 && p->ldy < p->n)), "%s: y is null, not 2-byte aligned or its row stride is less than n", me);
-    TLLM_REFUSE(p->rows && p->x == p->y, "%s: y lies where x does", me);
+    if (p->rows)
+    {
+        const int64_t tiles = (p->n + 15) / 16, groups = (p->k + p->group - 1) / p->group;
+        const Range y(p->y, (int64_t) p->n * 2, p->rows, p->ldy * 2);
+        TLLM_REFUSE(overlap(y, Range(p->x, (int64_t) p->k * 2, p->rows, p->ldx * 2)), "%s: y lies where x does", me);
+        TLLM_REFUSE(overlap(y, Range(p->packed, tiles * ((p->k + 127) / 128) * 1024)) || overlap(y, Range(p->scales, groups * tiles * 32)), "%s: y lies where the weights do", me);
+    }
     return true;
 }
 
