@@ -72,8 +72,8 @@ int32_t tllm_paged_plan(const tllm_paged_plan_params_t* p, tllm_stream_t stream)
  * input's type, NaN is stored as 0.  No slot twice in one call, and no two calls on one page at a time.
  * rot_dim > 0: dimensions 0 .. rot_dim of every key, and of every query if there are any, are rotated by rope[position]:
  * (cos, sin)[rot_dim / 2] of fp32, rope_len positions; pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) with rope_pairs = 1.  A row whose
- * position is not in the table is passed over.  The key is rounded once, from the rotated fp32 value to 8 bits.  q_out may be q; rows that are
- * passed over stay as they were.
+ * position is not in the table is passed over.  The key is rounded once, from the rotated fp32 value to 8 bits.  q_out may be q, with its strides, and lies on
+ * no place of q, k or v otherwise, nor with two rows on one place; rows that are passed over stay as they were.
  * Strides count elements; the last dimension is contiguous; k, v, q and q_out are 16-byte aligned with strides that are multiples of 8.
  * head_size 64, 128 or 256; rot_dim a multiple of 16, at most head_size; page_size as above; n_rows at most 2^19.
  * ---------------------------------------------------------------------------------------------- */
@@ -106,7 +106,7 @@ int32_t tllm_paged_append(const tllm_paged_append_params_t* p, tllm_stream_t str
  *   max_new  no request has more rows (rows behind that many are not computed);
  *   max_kv   an expectation of the longest kv_lens, for how the work is split; any kv_lens up to max_blocks * page_size is right.
  * Table entries that are no block of the pool count as masked.  Lengths beyond the table are cut to it.
- * out may be q itself, with its strides.
+ * out may be q itself, with its strides, and lies on no place of it otherwise, nor with two rows on one place.
  * At most 4096 requests and 2^19 rows; n_seqs * kv_heads * ceil(max_new * (q_heads / kv_heads) / 128) is at most 2^25 (64 for 128 with heads of 256): the work is
  * laid out as if every request had max_new rows, and what none has costs a workgroup's start.
  * Workspace: tllm_paged_attention_workspace() bytes, 16-byte aligned, not shared by calls that may overlap.

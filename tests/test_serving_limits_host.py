@@ -20,7 +20,7 @@ from test_serving_api_host import AT, attention_params
 ])
 def test_attention_takes_every_batch_that_a_launch_holds(n_seqs, n_rows, q_heads, kv_heads, size, max_new, fits):
     p = attention_params()
-    for name, v in dict(n_seqs=n_seqs, n_rows=n_rows, q_heads=q_heads, kv_heads=kv_heads, head_size=size, max_new=max_new, max_kv=100, q=AT).items():
+    for name, v in dict(n_seqs=n_seqs, n_rows=n_rows, q_heads=q_heads, kv_heads=kv_heads, head_size=size, max_new=max_new, max_kv=100, q_row=q_heads * size, q_head=size, out_row=q_heads * size, out_head=size).items():
         setattr(p, name, v)
     got = P._lib().tllm_paged_attention_workspace(ctypes.addressof(p))
     assert (got >= 0) == fits, capi.last_error()

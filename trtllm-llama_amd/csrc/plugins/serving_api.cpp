@@ -76,6 +76,53 @@ bool overlap(const Range& a, const Range& b)
     return false;
 }
 
+// [rows][heads][size] elements of 16 bits
+struct Rows
+{
+    int64_t at, bytes, rows, step, heads, head_step;
+    Rows(const void* p, int64_t rows, int64_t row, int32_t heads, int64_t head, int32_t size)
+        : at(static_cast<int64_t>(reinterpret_cast<uintptr_t>(p))), bytes(2 * (int64_t) size), rows(rows), step(rows > 1 ? 2 * row : 0), heads(heads),
+          head_step(heads > 1 ? 2 * head : 0)
+    {
+        if (heads > 1 && head_step == bytes)
+        {
+            bytes *= heads;
+            this->heads = 1;
+            head_step = 0;
+        }
+    }
+    Range head(int64_t i) const { return Range(reinterpret_cast<const void*>(static_cast<uintptr_t>(at + i * head_step)), bytes, rows, step); }
+    Range all() const
+    {
+        const int64_t r = (rows - 1) * step, h = (heads - 1) * head_step, low = at + std::min<int64_t>(r, 0) + std::min<int64_t>(h, 0);
+        return Range(reinterpret_cast<const void*>(static_cast<uintptr_t>(low)), std::max(r, -r) + std::max(h, -h) + bytes);
+    }
+    bool operator==(const Rows& o) const { return at == o.at && bytes == o.bytes && rows == o.rows && step == o.step && heads == o.heads && head_step == o.head_step; }
+};
+
+bool overlap(const Rows& a, const Rows& b)
+{
+    if (!overlap(a.all(), b.all()))
+        return false;
+    const bool apart = a.head_step == b.head_step; // only the distance counts
+    for (int64_t i = 0; i < (apart ? 1 : a.heads); ++i)
+        for (int64_t j = apart ? 1 - a.heads : 0; j < b.heads; ++j)
+            if (overlap(a.head(i), b.head(j)))
+                return true;
+    return false;
+}
+
+bool folded(const Rows& a) // two of its rows or heads share a place
+{
+    const Range first = a.head(0);
+    if (first.rows > 1 && first.step < first.bytes)
+        return true;
+    for (int64_t i = 1; i < a.heads; ++i)
+        if (overlap(first, a.head(i)))
+            return true;
+    return false;
+}
+
 constexpr int32_t kMaxRows = 1 << 19, kMaxHeads = 1024, kMaxTiles = 1 << 25;
 
 #define TLLM_REFUSE(cond, ...)                                                                                         \
@@ -157,8 +204,18 @@ bool append_fits(const tllm_paged_append_params_t* p)
         return true;
     TLLM_REFUSE(!p->slot_map || !aligned(p->slot_map, 4), "%s: the slot map is null or not 4-byte aligned", me);
     TLLM_REFUSE(p->rot_dim && (!p->positions || !aligned(p->positions, 4)), "%s: the positions are null or not 4-byte aligned", me);
-    return rows_fit(me, "k", p->k, p->k_row, p->k_head) && rows_fit(me, "v", p->v, p->v_row, p->v_head)
-        && (!p->q_heads || (rows_fit(me, "q", p->q, p->q_row, p->q_head) && rows_fit(me, "q_out", p->q_out, p->q_out_row, p->q_out_head)));
+    if (!rows_fit(me, "k", p->k, p->k_row, p->k_head) || !rows_fit(me, "v", p->v, p->v_row, p->v_head))
+        return false;
+    if (p->q_heads == 0)
+        return true;
+    if (!rows_fit(me, "q", p->q, p->q_row, p->q_head) || !rows_fit(me, "q_out", p->q_out, p->q_out_row, p->q_out_head))
+        return false;
+    const Rows out(p->q_out, p->n_rows, p->q_out_row, p->q_heads, p->q_out_head, p->head_size), q(p->q, p->n_rows, p->q_row, p->q_heads, p->q_head, p->head_size);
+    TLLM_REFUSE(folded(out), "%s: two rows of q_out lie on one place", me);
+    TLLM_REFUSE((!(out == q) && overlap(out, q)) || overlap(out, Rows(p->k, p->n_rows, p->k_row, p->kv_heads, p->k_head, p->head_size))
+            || overlap(out, Rows(p->v, p->n_rows, p->v_row, p->kv_heads, p->v_head, p->head_size)),
+        "%s: q_out lies across q, k or v", me);
+    return true;
 }
 
 bool attention_fits(const tllm_paged_attention_params_t* p)
@@ -181,7 +238,14 @@ bool attention_fits(const tllm_paged_attention_params_t* p)
     const int64_t rows = (int64_t) std::min(p->max_new, p->n_rows) * (p->q_heads / p->kv_heads), in_tile = p->head_size == 256 ? 64 : 128;
     TLLM_REFUSE((int64_t) p->n_seqs * p->kv_heads * ((rows + in_tile - 1) / in_tile) > kMaxTiles, "%s: %d requests of up to %d rows are more than one launch takes", me, p->n_seqs,
         p->max_new);
-    return p->n_rows == 0 || (rows_fit(me, "q", p->q, p->q_row, p->q_head) && rows_fit(me, "out", p->out, p->out_row, p->out_head));
+    if (p->n_rows == 0)
+        return true;
+    if (!rows_fit(me, "q", p->q, p->q_row, p->q_head) || !rows_fit(me, "out", p->out, p->out_row, p->out_head))
+        return false;
+    const Rows out(p->out, p->n_rows, p->out_row, p->q_heads, p->out_head, p->head_size), q(p->q, p->n_rows, p->q_row, p->q_heads, p->q_head, p->head_size);
+    TLLM_REFUSE(folded(out), "%s: two rows of out lie on one place", me);
+    TLLM_REFUSE(!(out == q) && overlap(out, q), "%s: out lies across q", me);
+    return true;
 }
 
 bool matmul_fits(const tllm_group_matmul_params_t* p)
