@@ -28,7 +28,7 @@ bool aligned(const void* p, size_t to)
 // `rows` pieces of `bytes`, one every `step` bytes
 struct Range
 {
-    int64_t at, bytes, rows, step;
+    int64_t at, bytes, rows, step, end; // of the last piece
     Range(const void* p, int64_t bytes, int64_t rows = 1, int64_t step = 0)
         : at(static_cast<int64_t>(reinterpret_cast<uintptr_t>(p))), bytes(bytes), rows(bytes > 0 ? rows : 0), step(step)
     {
@@ -44,8 +44,8 @@ struct Range
         }
         if (this->rows <= 1)
             this->step = 0;
+        end = at + (this->rows - 1) * this->step + this->bytes;
     }
-    int64_t end() const { return at + (rows - 1) * step + bytes; }
     bool operator==(const Range& o) const { return at == o.at && bytes == o.bytes && rows == o.rows && step == o.step; }
 };
 
@@ -62,18 +62,21 @@ bool meets(int64_t at, int64_t bytes, int64_t step, int64_t first, int64_t last,
     return std::max(first, floor_div(x - bytes - at, step) + 1) <= std::min(last, -floor_div(at - x - n, step) - 1);
 }
 
-bool overlap(const Range& a, const Range& b)
+bool pieces_meet(const Range& a, const Range& b)
 {
-    if (a.rows <= 0 || b.rows <= 0 || a.at >= b.end() || b.at >= a.end())
-        return false;
     if (a.rows > b.rows)
-        return overlap(b, a);
+        return pieces_meet(b, a);
     if (a.step == b.step) // only the distance counts
         return meets(b.at, b.bytes, b.step, 1 - a.rows, b.rows - 1, a.at, a.bytes);
     for (int64_t i = 0; i < a.rows; ++i)
         if (meets(b.at, b.bytes, b.step, 0, b.rows - 1, a.at + i * a.step, a.bytes))
             return true;
     return false;
+}
+
+inline bool overlap(const Range& a, const Range& b)
+{
+    return a.at < b.end && b.at < a.end && a.rows > 0 && b.rows > 0 && pieces_meet(a, b);
 }
 
 // [rows][heads][size] elements of 16 bits

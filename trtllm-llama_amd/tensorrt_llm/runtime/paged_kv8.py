@@ -51,11 +51,8 @@ def on_device(index: int, call, *args):
         torch.cuda.set_device(current)
 
 
-def packed(layout: struct.Struct, *values) -> bytes:
-    try:
-        return layout.pack(*values)
-    except (struct.error, OverflowError, TypeError) as e:
-        raise ValueError(f'an argument is no number of its kind: {e}') from None
+def _no_number(e):
+    raise ValueError(f'an argument is no number of its kind: {e}') from None
 
 
 def _raise(name):
@@ -136,8 +133,11 @@ def plan_step(lens: torch.Tensor, new_lens: torch.Tensor, ring: torch.Tensor, ri
         raise ValueError(f'out is a plan of {out.n_seqs} requests and {out.n_rows} rows on GPU {out.index}, the step has {n} and {n_rows} on GPU {index}')
     table, stride, wide = _table(block_table, n, index)
     blocks = ring.numel()
-    p = packed(_PLAN, n, n_rows, page_size, blocks, wide, stride, _ints('lens', lens, n, index), _ints('new_lens', new_lens, n, index), _ints('ring', ring, blocks, index),
-               _ints('ring_state', ring_state, 2, index), table, *out._at)
+    try:
+        p = _PLAN.pack(n, n_rows, page_size, blocks, wide, stride, _ints('lens', lens, n, index), _ints('new_lens', new_lens, n, index), _ints('ring', ring, blocks, index),
+                       _ints('ring_state', ring_state, 2, index), table, *out._at)
+    except struct.error as e:
+        _no_number(e)
     if on_device(index, (_lib_ or _lib()).tllm_paged_plan, p):
         _raise('plan_step')
     return out
@@ -230,8 +230,11 @@ class PagedKV8Cache(Fixed):
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             o_at, _, o_row, o_head = _rows('q_out', q_out, rows, q_heads, size, dtype, index, True)
-        p = packed(_APPEND, rows, heads, q_heads, size, self.page_size, self.blocks, act, self._type, rot, 1 if rope_pairs else 0, angle_rows, k_at, v_at, q_at, o_at,
-                   k_row, k_head, v_row, v_head, q_row, q_head, o_row, o_head, _ints('slot_map', slot_map, rows, index), places, angles, *self._at)
+        try:
+            p = _APPEND.pack(rows, heads, q_heads, size, self.page_size, self.blocks, act, self._type, rot, 1 if rope_pairs else 0, angle_rows, k_at, v_at, q_at, o_at,
+                             k_row, k_head, v_row, v_head, q_row, q_head, o_row, o_head, _ints('slot_map', slot_map, rows, index), places, angles, *self._at)
+        except struct.error as e:
+            _no_number(e)
         if on_device(index, (_lib_ or _lib()).tllm_paged_append, p):
             _raise('append')
         return q_out
@@ -251,9 +254,12 @@ class PagedKV8Cache(Fixed):
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         o_at, _, o_row, o_head = _rows('out', out, rows, heads, size, dtype, index, True)
-        p = packed(_ATTENTION, n, rows, heads, self.kv_heads, size, self.page_size, self.blocks, wide, act, self._type, max_new,
-                   wide * self.page_size if max_kv is None else max_kv, window, size**-0.5 if scale is None else scale, stride, q_row, q_head, o_row, o_head,
-                   q_at, *self._at, table, _ints('cu_tokens', cu_tokens, n + 1, index), _ints('kv_lens', kv_lens, n, index), o_at)
+        try:
+            p = _ATTENTION.pack(n, rows, heads, self.kv_heads, size, self.page_size, self.blocks, wide, act, self._type, max_new,
+                                wide * self.page_size if max_kv is None else max_kv, window, size**-0.5 if scale is None else scale, stride, q_row, q_head, o_row, o_head,
+                                q_at, *self._at, table, _ints('cu_tokens', cu_tokens, n + 1, index), _ints('kv_lens', kv_lens, n, index), o_at)
+        except struct.error as e:
+            _no_number(e)
         if on_device(index, self._attend, p):
             _raise('attention')
         return out
