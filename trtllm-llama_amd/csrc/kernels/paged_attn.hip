@@ -324,8 +324,8 @@ __device__ __forceinline__ void rows_body(const tllm_paged_attention_params_t& p
     for (int i = 0; i < kOut; ++i)
         o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     Seen row_seen;
-    // The last tile of a wave sends for nothing.  It is a body of its own: with the loads under a condition inside one loop the compiler's scheduler
-    // has written over registers of the values that were still to be read (hipcc 7.2, seen in the assembly and by the tests).
+    // The last tile of a wave sends for nothing.  It is a body of its own: with the loads under a condition inside one loop hipcc 7.2 takes registers of the
+    // values that are still to be read for the exponentials (heads of 64, behind `cut`); a test looks for that in the assembly.
     auto step = [&](int t, auto more) {
         const int vk = t * kTile + 16 * g;
         const bool v_in = held(vb_now);
