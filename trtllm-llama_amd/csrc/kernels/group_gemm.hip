@@ -5,7 +5,8 @@
 // A k-step is 32 consecutive k of every row, so it lies in one group whatever the group's size; the products of a group are summed by
 // themselves and enter the result times the scale in fp32: neither weight nor scale is rounded on the way.
 // fp16: nibbles to 1024 + u and 1024 + 16 u by a mask, then u - 8 exactly by a packed subtraction or FMA.  bfloat16 has no packed arithmetic:
-// 128 + u goes into the product as it is, and 136 times the sum of the group's x - one more product, with ones for weights - comes off.
+// 128 + u goes into the product as it is, and 136 times the sum of the group's x - one more product, with ones for weights - comes off; the difference is up
+// to 2^5 smaller than the two, so that it keeps 19 of fp32's 24 bits, where the result keeps 8, and a row with values from 2^113 on comes out as NaN.
 #include "dev_utils.h"
 #include "launch_util.h"
 #include "serving_kernels.h"
@@ -426,7 +427,9 @@ void launch_few(const tllm_group_matmul_params_t& p, hipStream_t stream)
 }
 
 // The forms and what a workgroup takes in each (us, all CUs busy): `once` and `each` k-tile, fitted to 256 and 1024 workgroups of fp16 with groups
-// of 128 over k of 512 to 11008, which they meet within 10 %.  A product takes as many rounds as its workgroups take CUs, and the form with the
+// of 128 over k of 512 to 11008, which they meet within 10 %; a launch, 1 to 2 us, comes on top (64 x 12288 x 4096: 11.9 by the table, 14.1 measured).  Other types
+// and groups choose by the same table, which was not fitted to them: 1024 x 11008 x 4096 takes 112 us, bfloat16 117, with groups of 64 142, of 32 191, and in the
+// form 64 x 48, where small groups have no registers left, 128 x 11008 x 4096 takes 26, bfloat16 26, with groups of 64 45, of 32 166.  A product takes as many rounds as its workgroups take CUs, and the form with the
 // least time is the one to take: 1 x 4096 x 4096 in 256 workgroups of 16 outputs, 1024 x 11008 x 4096 in 464 tiles of 128 x 192 (109 us; 126 in tiles of
 // 128, 136 in tiles of 256, 197 in tiles of 64), 1024 x 4096 x 4096 in 256 of 128 x 128 (44 us; 54 in tiles of 192), 67 x 190 x 10144 in 204 of 4 x 16 (6.5 us; 143 in
 // tiles of 192).

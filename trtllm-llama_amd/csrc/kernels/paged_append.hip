@@ -355,7 +355,9 @@ void launch_dim(const tllm_paged_append_params_t& p, hipStream_t stream)
     // Rows a workgroup looks for runs in.  The host does not know whether they are tokens (a run each, that want workgroups of their own) or
     // prompts (a run a page, where workgroups without one are most of the time): one row while that makes few workgroups, up to 16 where the
     // chip is full of them either way, a page where that leaves thousands (us at 1 / 8 / 16 / 64 rows, 8 heads of 128: 64 tokens 8 / 25 / 44 / 168,
-    // 512 tokens 42 / 34 / 52 / 178, a prompt of 1024 74 / 26 / 18 / 12, prompts of 5459 82 / 32 / 34 / 32)
+    // 512 tokens 42 / 34 / 52 / 178, a prompt of 1024 74 / 26 / 18 / 12, prompts of 5459 82 / 32 / 34 / 32).  Rows times heads are taken for a prompt, and
+    // tokens that make as many pay for it, a run behind the other: 64 tokens of 32 heads 19 us, 128 34, 1024 255 (a prompt of as many 23), 64 beside a
+    // prompt of 1024 190.
     const int64_t work = (int64_t) p.n_rows * p.kv_heads;
     int chunk = 1;
     while (chunk * 2 <= std::min(16, p.page_size) && chunk * 2 * 512 <= work)

@@ -20,8 +20,8 @@
 //               softmax -> join).
 //   tile_kernel 64 or 128 rows: the waves share the tiles, which they bring to LDS as fp16 fragments, the next one while this one is computed.  Prompts
 //               are bound by the arithmetic - products, exponentials, and the conversions, which are once a workgroup here and not once a wave: 0.90
-//               PFLOP/s where workgroups fill the chip evenly (2048 tokens behind 20000, 32 heads of 128), 0.62 where 640 of them have 512 places (three
-//               prompts of up to 1024 behind up to 2500: 184 us).
+//               PFLOP/s where workgroups fill the chip evenly (2048 tokens behind 20000, 32 heads of 128), 0.63 where 640 of them have 512 places (three
+//               prompts of up to 1024 behind up to 2500: 182 us).
 #include "dev_utils.h"
 #include "launch_util.h"
 #include "serving_kernels.h"
@@ -460,7 +460,7 @@ struct TileForm
     static constexpr int kKeyFrags = 4 * DIM / 32, kFrags = 2 * kKeyFrags; // of 1 KB: keys [part][k-step], values [channels / 16][k-step]
     static constexpr int kAhead = DIM == 256 ? 2 : 4; // fragments that are read ahead of their products
     // Tiles that LDS holds: two, one computed and one arriving; of heads of 256 one, so that two workgroups fit a CU (with some 30 registers a lane
-    // spilled; 1024 tokens behind 1500, 32 heads: 105 us, one workgroup a half more)
+    // spilled; 1024 tokens behind 1500, 32 heads: 98 us, one workgroup a half more)
     static constexpr int kBuffers = DIM == 256 ? 1 : 2, kLds = kBuffers * kFrags * 1024;
 };
 
