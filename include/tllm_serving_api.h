@@ -104,6 +104,7 @@ int32_t tllm_paged_append(const tllm_paged_append_params_t* p, tllm_stream_t str
  * scale >= 0.  Scores, softmax and sums in fp32.  Two things are rounded on the way: the weights enter the second product as fp16, each to 2^-11 of itself, or to
  * 2^-32 of the row's largest product of weight and page's value scale where its own is below 2^-21 of that; bfloat16 queries enter the first one as fp16 under a
  * power of two per row, exactly down to 2^-17 of the row's largest value and to 2^-25 of it below.  What a row does not see has no part in either.
+ * Scores are below 2^24 in magnitude (fp32 has no fraction beyond); a row with larger ones may be NaN.
  *   max_new  no request has more rows (rows behind that many are not computed);
  *   max_kv   an expectation of the longest kv_lens, for how the work is split; any kv_lens up to max_blocks * page_size is right.
  * Table entries that are no block of the pool count as masked.  Lengths beyond the table are cut to it.

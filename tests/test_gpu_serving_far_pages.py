@@ -107,3 +107,26 @@ def test_keys_of_nothing_in_a_page_of_the_largest(lens, rows, max_kv, size):
     cache.scales[:, 0] = float(torch.finfo(torch.bfloat16).max) / 127
     q = torch.from_numpy(rng.standard_normal((sum(rows), 2, size)).astype(np.float32) * 2.0**20).bfloat16()
     check(cache, q, 'bf16', lens, rows, max_kv=max_kv)
+
+
+@pytest.mark.parametrize('size', [64, 128, 256])
+@pytest.mark.parametrize('lens,rows,max_kv', SPANS)
+@pytest.mark.parametrize('loud', [2.0**8, 2.0**14])
+def test_large_scores_that_are_equal(lens, rows, max_kv, size, loud):
+    """Every key the same: weights are equal whatever the scores are (here up to some 2^22), and what rounding does to a score it does to the sum as well.  Off by the
+    weights' rounding, the sums' and the result's."""
+    rng = np.random.default_rng(size + 4)
+    cache = cache_of(rng, sum(-(-n // PAGE) for n in lens), size)
+    cache.pool[:, 0] = torch.from_numpy(rng.integers(64, 128, size).astype(np.int8)).cuda().repeat(PAGE)
+    cache.scales[:, 0] = 0.0173
+    cache.scales[:, 1] = 0.0119
+    q = torch.from_numpy((rng.uniform(0.5, 1, (sum(rows), 2, size)) * rng.choice([-1, 1], (sum(rows), 2, 1)) * loud).astype(np.float32)).bfloat16()
+    table, at = np.zeros((len(lens), -(-max(lens) // PAGE)), np.int32), 0
+    for b, n in enumerate(lens):
+        have = -(-n // PAGE)
+        table[b, :have] = np.arange(at, at + have)
+        at += have
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    got = numbers(cache.attention(q.cuda(), gpu(table), gpu(cu), gpu(lens), max(rows), max_kv))
+    want, spread, _ = O.attention(np.zeros(q.shape), cache.pool.cpu().float().numpy(), cache.scales.cpu().numpy(), table, cu, lens, PAGE, 1.0)
+    assert (np.abs(got - want) <= (2.0**-11 + 2.0**-17) * spread * 1.01 + HALF['bf16'] * np.abs(want) * 1.01).all()

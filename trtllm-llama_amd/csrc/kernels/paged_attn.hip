@@ -20,8 +20,8 @@
 //               softmax -> join).
 //   tile_kernel 64 or 128 rows: the waves share the tiles, which they bring to LDS as fp16 fragments, the next one while this one is computed.  Prompts
 //               are bound by the arithmetic - products, exponentials, and the conversions, which are once a workgroup here and not once a wave: 0.90
-//               PFLOP/s where workgroups fill the chip evenly (2048 tokens behind 20000, 32 heads of 128), 0.63 where 640 of them have 512 places (three
-//               prompts of up to 1024 behind up to 2500: 182 us).
+//               PFLOP/s where workgroups fill the chip evenly (2048 tokens behind 20000, 32 heads of 128), 0.64 where 640 of them have 512 places (three
+//               prompts of up to 1024 behind up to 2500: 178 us).
 #include "dev_utils.h"
 #include "launch_util.h"
 #include "serving_kernels.h"
@@ -192,7 +192,7 @@ __device__ __forceinline__ float part_of(float mine, float all) // exp2(mine - a
 }
 __device__ __forceinline__ float result_of(float m, float mv, float l) // of O; a row that saw nothing is 0, a NaN stays one
 {
-    return (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) * part_of(mv - kPShift, m);
+    return (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) * (part_of(mv, m) * __builtin_amdgcn_exp2f(-kPShift));
 }
 
 // One tile of one row: the 16 scores of a lane (keys key0 .. + 15 of a query's row), under the key scale `ks` of their page and log2 of its value scale `lv` -> its weights in fp16, with what
@@ -200,19 +200,20 @@ __device__ __forceinline__ float result_of(float m, float mv, float l) // of O; 
 template <int N>
 __device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], Seen& r, f32x4 (&o)[N], float ks, float lv, float factor, bool plain, bool in, int key0, int from, int seen)
 {
-    float f = fminf(factor * ks, 3.4028235e38f); // zero keys under the largest scale score 0, not 0 times an infinity
+    // zero keys under the largest scale score 0, not 0 times an infinity, and masked ones -INFINITY, not 0 times that
+    const float f = fminf(fmaxf(factor * ks, 1.17549435e-38f), 3.4028235e38f);
     if (!plain)
     {
+        const int begin = from - key0, end = in ? seen - key0 : -1;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            s[i] = in && key0 + i < seen && key0 + i >= from ? s[i] * f : -INFINITY;
-        f = 1.f;
+            s[i] = i < end && i >= begin ? s[i] : -INFINITY;
     }
     float top = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i)
         top = fmaxf(top, s[i]);
-    top *= f; // f >= 0
+    top *= f; // f > 0
     const float top_v = top + lv;
     if (__builtin_amdgcn_ballot_w64(top > r.m + kSlack || top_v > r.mv + kSlack))
     {
@@ -225,18 +226,18 @@ __device__ __forceinline__ void soften(float (&s)[16], f16x8 (&w)[2], Seen& r, f
         for (int i = 0; i < N; ++i)
             o[i] *= back;
     }
-    // weights are exp2(score + lift).  Where that would be below 2^-60 they are 0 in fp16 either way, and only l has to see them
-    const float m = r.m == -INFINITY ? 0.f : r.m, lift = fmaxf(lv - (r.mv == -INFINITY ? 0.f : r.mv), -60.f - m) + kPShift;
+    // weights are exp2(score - m + lift).  Where that would be below 2^-60 they are 0 in fp16 either way, and only l has to see them
+    const float m = r.m == -INFINITY ? 0.f : r.m, lift = fmaxf(lv - ((r.mv == -INFINITY ? 0.f : r.mv) - m), -60.f) + kPShift, shift = lift - m;
     float sum = 0.f;
     u32x4 p[2];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
     {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], f, lift)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], f, lift));
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], f, shift)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], f, shift));
         sum += a + b;
         p[i >> 2][i & 3] = pack_f16(a, b);
     }
-    r.l += sum * __builtin_amdgcn_exp2f(-lift - m);
+    r.l += sum * __builtin_amdgcn_exp2f(-lift);
     w[0] = join(p[0]);
     w[1] = join(p[1]);
 }
@@ -459,7 +460,7 @@ struct TileForm
     static constexpr int kRt = DIM == 256 ? 1 : 2, kRows = 64 * kRt; // row tiles of a wave, rows of a workgroup of four
     static constexpr int kKeyFrags = 4 * DIM / 32, kFrags = 2 * kKeyFrags; // of 1 KB: keys [part][k-step], values [channels / 16][k-step]
     static constexpr int kAhead = DIM == 256 ? 2 : 4; // fragments that are read ahead of their products
-    // Tiles that LDS holds: two, one computed and one arriving; of heads of 256 one, so that two workgroups fit a CU (with some 30 registers a lane
+    // Tiles that LDS holds: two, one computed and one arriving; of heads of 256 one, so that two workgroups fit a CU (with 30 to 60 registers a lane
     // spilled; 1024 tokens behind 1500, 32 heads: 98 us, one workgroup a half more)
     static constexpr int kBuffers = DIM == 256 ? 1 : 2, kLds = kBuffers * kFrags * 1024;
 };
